@@ -307,6 +307,24 @@ int mek_conv1d_bwd(const void* x, const void* x_prev, const void* x_next, const 
                    const void* dy, const void* dy_next, const uint8_t* reach, void* dx, void* dw_partial, void* dw,
                    int fp32_policy, int tokens, int channels, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * LayerNorm over rows of any width, forward and backward:
+ *     unit = (x - mean(x)) / sqrt(var(x) + eps),   y = unit weight + bias
+ * Element types: 0 bf16, 1 fp16, 2 fp32.  x [rows, width] of `type` with x_row_stride elements between rows and unit
+ * stride inside one; y, dy, dx dense of the same type; weight, bias, dw, db [width] of `param_type`, each or NULL
+ * (NULL weight: ones, NULL bias: zeros); mean, rstd fp32 [rows] (or NULL: not written); codes uint8 [rows, width]: unit
+ * in e4m3, the 8-bit checkpoint (or NULL; width <= 200,704, the widest row whose values cannot exceed the format).
+ * The backward takes unit from codes, or from x and mean where codes is NULL.  dw and db (each or NULL) are summed in
+ * a fixed order: FP32 per block into partial fp32 [mek_layer_norm_partial_rows(rows, width, type), 2, width] (NULL
+ * with both NULL), then FP64 over the blocks.  No counterpart in the reference. */
+int mek_layer_norm_partial_rows(int64_t rows, int64_t width, int type);
+int mek_layer_norm_fwd(const void* x, int type, const void* weight, const void* bias, int param_type, void* y,
+                       float* mean, float* rstd, uint8_t* codes, int64_t rows, int64_t width, int64_t x_row_stride,
+                       float eps, void* stream);
+int mek_layer_norm_bwd(const void* dy, const void* x, int type, const uint8_t* codes, const float* mean,
+                       const float* rstd, const void* weight, int param_type, void* dx, float* partial, void* dw,
+                       void* db, int64_t rows, int64_t width, int64_t x_row_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

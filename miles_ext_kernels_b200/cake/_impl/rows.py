@@ -1,0 +1,46 @@
+"""What the row operators (LayerNorm, the gated norm's checkpoint, the linear recurrence) share on the host: element
+types as the C ABI numbers them, checkpoint formats, the device check and the device guard."""
+
+from __future__ import annotations
+
+from contextlib import nullcontext
+from typing import Any
+
+import torch
+
+from .._runtime import loader
+
+__all__ = ["CHECKPOINTS", "TYPES", "check_device", "checkpoint_format", "on_device"]
+
+# element types of the C ABI
+TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# how a forward may keep what its backward needs: as it came, or in 8 bits
+CHECKPOINTS = (None, "e4m3")
+
+_NOTHING = nullcontext()
+
+
+def on_device(device: torch.device) -> Any:
+    """``torch.cuda.device(device)``, without its cost where ``device`` is the current one."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NOTHING
+    return torch.cuda.device(device)
+
+
+def checkpoint_format(op: str, checkpoint: Any) -> bool:
+    """Whether ``checkpoint`` asks for e4m3 codes; ``ValueError`` for anything but the formats of ``CHECKPOINTS``."""
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"{op}: checkpoint must be one of {CHECKPOINTS}, got {checkpoint!r}")
+    return checkpoint is not None
+
+
+def check_device(op: str, what: str, device: Any = None) -> None:
+    """Raise ``ValueError`` unless the kernels run on ``device`` (default: the current CUDA device)."""
+    served = tuple(loader.ARCH_BY_CAPABILITY)
+    if not torch.cuda.is_available():
+        raise ValueError(f"{op} needs a CUDA device of compute capability {served}")
+    capability = tuple(torch.cuda.get_device_capability(device))
+    arch = loader.ARCH_BY_CAPABILITY.get(capability)
+    if arch is None:
+        raise ValueError(f"{op} runs on compute capability {served}, not {capability}")
+    loader.check_toolkit(arch, what)

@@ -2,7 +2,8 @@
 
 :data:`OPS` names every ``cake/<op>.py`` of this package.  :func:`op_spec` imports only the thin op module, never
 its implementation (reference: miles_ext_kernels/cake/_runtime/registry.py:26-158; the reference lists 13 ops, this
-package ships the two of the gated-delta-rule path).
+package ships those of the gated-delta-rule path and, without a counterpart there, the other ops of a recurrent
+layer's training path).
 """
 
 from __future__ import annotations
@@ -18,7 +19,7 @@ from .spec import OpSpec
 
 __all__ = ["OPS", "op_spec", "prebuild", "release"]
 
-OPS: tuple[str, ...] = ("gdn", "kda", "gated_rmsnorm", "conv1d")
+OPS: tuple[str, ...] = ("gdn", "kda", "gated_rmsnorm", "conv1d", "layer_norm")
 
 # <pkg>.cake: op modules are its submodules, implementations those of its _impl package
 _SOURCE = __name__.rsplit(".", 2)[0]

@@ -1,0 +1,93 @@
+// Element types, vector loads and the 8-bit checkpoint format of the row operators (LayerNorm, the gated norm's
+// checkpoint, the linear recurrence).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <stdint.h>
+
+namespace mek {
+
+enum : int { kTypeBf16 = 0, kTypeFp16 = 1, kTypeFp32 = 2 };
+
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+
+// N neighbouring elements of T moved as one access.
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T e[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Vec<T, N>& raw, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = to_float(raw.e[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> pack(const float (&v)[N]) {
+  Vec<T, N> raw;
+#pragma unroll
+  for (int i = 0; i < N; ++i) raw.e[i] = from_float<T>(v[i]);
+  return raw;
+}
+
+// Element i of a parameter vector in one of the three types (a launch-uniform switch).
+__device__ __forceinline__ float load_param(const void* p, int type, int64_t i) {
+  if (type == kTypeBf16) return to_float(static_cast<const __nv_bfloat16*>(p)[i]);
+  if (type == kTypeFp16) return to_float(static_cast<const __half*>(p)[i]);
+  return static_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store_param(void* p, int type, int64_t i, float v) {
+  if (type == kTypeBf16) static_cast<__nv_bfloat16*>(p)[i] = from_float<__nv_bfloat16>(v);
+  else if (type == kTypeFp16) static_cast<__half*>(p)[i] = from_float<__half>(v);
+  else static_cast<float*>(p)[i] = v;
+}
+
+// e4m3 codes (4 exponent bits, 3 mantissa bits, largest 448, NaN but no infinity), rounded to nearest even: off by at
+// most 2^-4 of the value for magnitudes in [2^-6, 448], by 2^-10 below.
+template <int N>
+__device__ __forceinline__ Vec<uint8_t, N> to_e4m3(const float (&v)[N]) {
+  Vec<uint8_t, N> out;
+  if constexpr (N == 1) {
+    out.e[0] = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
+      out.e[i] = uint8_t(two & 0xff), out.e[i + 1] = uint8_t(two >> 8);
+    }
+  }
+  return out;
+}
+template <int N>
+__device__ __forceinline__ void from_e4m3(const Vec<uint8_t, N>& codes, float (&v)[N]) {
+  if constexpr (N == 1) {
+    v[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(codes.e[0], __NV_E4M3)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const __nv_fp8x2_storage_t two = __nv_fp8x2_storage_t(codes.e[i] | (codes.e[i + 1] << 8));
+      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+      v[i] = f.x, v[i + 1] = f.y;
+    }
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  return x;
+}
+
+}  // namespace mek
