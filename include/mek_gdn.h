@@ -325,6 +325,35 @@ int mek_layer_norm_bwd(const void* dy, const void* x, int type, const uint8_t* c
                        const float* rstd, const void* weight, int param_type, void* dx, float* partial, void* dw,
                        void* db, int64_t rows, int64_t width, int64_t x_row_stride, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------
+ * Gated linear recurrence per channel, forward, backward and the single-token step:
+ *     h[t] = exp(g[t]) h[t-1] + x[t],   y[t] = h[t]
+ * x, g [batch, tokens, channels] of x_type / g_type (0 bf16, 1 fp16, 2 fp32), unit stride over the channels, any
+ * strides (elements) between tokens and batch rows; y, dy, dx (x_type) and dg (g_type) dense.  With cu_seqlens (int32
+ * [num_seqs + 1] on the device, batch = 1) the tokens are packed sequences; y, dx, dg of tokens outside
+ * [cu_seqlens[0], cu_seqlens[num_seqs]) are zero.  States fp32 [sequences, channels], each optional: initial_state
+ * (NULL: zero), final_state, d_final_state (NULL: zero), dh0; a sequence without tokens passes its state through.
+ * More than mek_linear_recurrence_tile() tokens need scratch fp32 [2, batch, tiles, channels] (backward: [3, ...])
+ * with tiles = ceil(tokens / tile) and ends fp32 [batch, tiles, channels], the state after every tile, which the
+ * backward reads.  step: one token of every row on a pool of states fp32 [pool, channels] (state_row_stride elements
+ * between them), updated in place: row r uses state slots[r] (int32, or int64 when slots_are_int64; NULL: r); a slot
+ * outside [0, pool) leaves every state alone and gives zeros; rows that name one slot take their turns in row order.
+ * No counterpart in the reference. */
+int mek_linear_recurrence_tile(void);
+int mek_linear_recurrence_fwd(const void* x, int x_type, const void* g, int g_type, void* y, int64_t batch,
+                              int64_t tokens, int64_t channels, int64_t x_batch_stride, int64_t x_token_stride,
+                              int64_t g_batch_stride, int64_t g_token_stride, const int32_t* cu_seqlens, int64_t num_seqs,
+                              const float* initial_state, float* final_state, float* scratch, float* ends,
+                              void* stream);
+int mek_linear_recurrence_bwd(const void* dy, const void* x, int x_type, const void* g, int g_type, void* dx, void* dg,
+                              int64_t batch, int64_t tokens, int64_t channels, int64_t x_batch_stride,
+                              int64_t x_token_stride, int64_t g_batch_stride, int64_t g_token_stride,
+                              const int32_t* cu_seqlens, int64_t num_seqs, const float* initial_state,
+                              const float* d_final_state, const float* ends, float* dh0, float* scratch, void* stream);
+int mek_linear_recurrence_step(const void* x, int x_type, const void* g, int g_type, float* state, const void* slots,
+                               int slots_are_int64, void* y, int64_t rows, int64_t pool, int64_t channels,
+                               int64_t x_row_stride, int64_t g_row_stride, int64_t state_row_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

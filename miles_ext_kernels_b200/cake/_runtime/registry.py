@@ -19,7 +19,7 @@ from .spec import OpSpec
 
 __all__ = ["OPS", "op_spec", "prebuild", "release"]
 
-OPS: tuple[str, ...] = ("gdn", "kda", "gated_rmsnorm", "conv1d", "layer_norm")
+OPS: tuple[str, ...] = ("gdn", "kda", "gated_rmsnorm", "conv1d", "layer_norm", "linear_recurrence")
 
 # <pkg>.cake: op modules are its submodules, implementations those of its _impl package
 _SOURCE = __name__.rsplit(".", 2)[0]

@@ -1,10 +1,11 @@
-"""Plain 64-bit forms of the row operators, written from their definitions: LayerNorm and its 8-bit checkpoint."""
+"""Plain 64-bit forms of the row operators, written from their definitions: LayerNorm and its 8-bit checkpoint, the gated
+linear recurrence."""
 
 from __future__ import annotations
 
 import torch
 
-__all__ = ["U32", "e4m3_misses", "half_step", "layer_norm", "layer_norm_bwd", "misses"]
+__all__ = ["U32", "e4m3_misses", "half_step", "layer_norm", "layer_norm_bwd", "linear_recurrence", "misses"]
 
 U32 = 2.0**-24  # half a step of FP32, relative
 
@@ -65,3 +66,51 @@ def layer_norm_bwd(dy, unit, rstd, weight, unit_slack):
     dw, db = (dy * unit).sum(0), dy.sum(0)
     dw_slack = 512 * U32 * (dy * unit).abs().sum(0) + (dy.abs() * unit_slack).sum(0)
     return {"dx": (dx, dx_slack), "dw": (dw, dw_slack), "db": (db, 512 * U32 * dy.abs().sum(0))}
+
+
+def linear_recurrence(x, g, lengths, h0=None, dy=None, d_final=None):
+    """``{name: (value, slack)}`` of the packed tokens ``x``, ``g [T, C]`` of consecutive sequences of ``lengths``, token by
+    token in 64 bits.  The slack follows the sizes: with m the sum of magnitudes that the state could have (no
+    cancellation), a step adds at most 6 half steps of FP32 to what it carries over -- a decay within 3 half steps of
+    exp(g), its product and the fold's -- and 2 to the new state.  A decay below e^-87 counts as zero, which takes away
+    less than e^-87 = 1.65e-38 of what the step carries over (g < -87 <=> exp(g) < e^-87)."""
+    total, channels = x.shape
+    x, a = x.double(), g.double().exp()
+    n = len(lengths)
+    h0 = x.new_zeros(n, channels) if h0 is None else h0.double()
+    y, dy_slack = torch.zeros_like(x), torch.zeros_like(x)
+    before, before_slack = torch.zeros_like(x), torch.zeros_like(x)
+    final, final_slack = h0.clone(), torch.zeros_like(h0)
+    start = 0
+    spans = []
+    for i, length in enumerate(lengths):
+        spans.append((start, start + length))
+        h, m, e = h0[i], h0[i].abs(), torch.zeros_like(h0[i])
+        for t in range(start, start + length):
+            before[t], before_slack[t] = h, e
+            e = a[t] * (e + 6 * U32 * m) + 1.65e-38 * m
+            h, m = a[t] * h + x[t], a[t] * m + x[t].abs()
+            e = e + 2 * U32 * m
+            y[t], dy_slack[t] = h, e
+        final[i], final_slack[i] = h, e
+        start += length
+    out = {"y": (y, dy_slack), "final": (final, final_slack)}
+    if dy is None:
+        return out
+    dy = dy.double()
+    d_final = torch.zeros_like(h0) if d_final is None else d_final.double()
+    dx, dg, dx_slack, dg_slack = (torch.zeros_like(x) for _ in range(4))
+    dh0, dh0_slack = d_final.clone(), torch.zeros_like(h0)
+    for i, (lo, hi) in enumerate(spans):
+        c, m, e = d_final[i], d_final[i].abs(), torch.zeros_like(d_final[i])
+        for t in range(hi - 1, lo - 1, -1):
+            dh, m = dy[t] + c, dy[t].abs() + m
+            e = e + 2 * U32 * m
+            dx[t], dx_slack[t] = dh, e
+            c = a[t] * dh
+            e, m = a[t] * (e + 6 * U32 * m) + 1.65e-38 * m, a[t] * m
+            dg[t] = c * before[t]
+            dg_slack[t] = e * before[t].abs() + c.abs() * before_slack[t] + e * before_slack[t] + 4 * U32 * dg[t].abs()
+        dh0[i], dh0_slack[i] = c, e
+    out.update(dx=(dx, dx_slack), dg=(dg, dg_slack), dh0=(dh0, dh0_slack))
+    return out
