@@ -282,6 +282,18 @@ int mek_gated_rmsnorm_bwd(const void* dy, const void* x, const void* z, const vo
                           float* dw_partial, void* dw, int64_t rows, int heads, int64_t x_token_stride,
                           int64_t x_head_stride, int64_t z_token_stride, int64_t z_head_stride, float eps,
                           void* stream);
+/* The same with an 8-bit checkpoint: fwd_keep also writes, per row, n = x rstd as e4m3 codes (n_codes uint8 [rows, 128]),
+ * z 2^-e as e4m3 codes (z_codes) under the smallest e >= -126 that brings the row's largest finite magnitude to at
+ * most 448 (z_exponent uint8 [rows]: e + 127; a value that is not finite becomes NaN) and rstd (fp32 [rows]); y has the
+ * bits of mek_gated_rmsnorm_fwd.  bwd_kept takes n and z from the codes: x and z need not be kept.  No counterpart in
+ * the reference. */
+int mek_gated_rmsnorm_fwd_keep(const void* x, const void* z, const void* weight, void* y, uint8_t* n_codes,
+                               uint8_t* z_codes, uint8_t* z_exponent, float* rstd, int64_t rows, int heads,
+                               int64_t x_token_stride, int64_t x_head_stride, int64_t z_token_stride,
+                               int64_t z_head_stride, float eps, void* stream);
+int mek_gated_rmsnorm_bwd_kept(const void* dy, const uint8_t* n_codes, const uint8_t* z_codes,
+                               const uint8_t* z_exponent, const float* rstd, const void* weight, void* dx, void* dz,
+                               float* dw_partial, void* dw, int64_t rows, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------------
  * Packed causal depthwise conv1d (kernel size 4) + SiLU, the short convolution in front of the GDN / KDA op:

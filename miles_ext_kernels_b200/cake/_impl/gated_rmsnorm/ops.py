@@ -7,9 +7,10 @@ head strides) and a BF16 ``weight [128]`` shared by every token and head::
     rstd = 1 / sqrt(mean(x^2) + eps)                     # FP32
     y    = bf16(((x * rstd) * weight) * silu(z))         # FP32, one rounding
 
-The autograd node saves only ``x``, ``z`` and ``weight``; the backward recomputes ``rstd``.  The weight gradient is
-summed in FP32 per block and in FP64 across the blocks, in an order fixed by the row count: the same bits on every
-call, in either variant.
+The autograd node saves only ``x``, ``z`` and ``weight``; the backward recomputes ``rstd``.  With ``checkpoint="e4m3"`` it
+saves ``x * rstd`` and ``z`` as 8-bit codes instead, half the bytes, and the backward takes both rounded to 3 mantissa
+bits.  The weight gradient is summed in FP32 per block and in FP64 across the blocks, in an order fixed by the row
+count: the same bits on every call, in either variant.
 """
 
 from __future__ import annotations
@@ -21,6 +22,7 @@ import torch
 
 from ..._runtime import config, loader, registry, workspace
 from ..gdn import native
+from ..rows import checkpoint_format
 
 __all__ = ["check_supported", "prebuild", "release", "rmsnorm_silu_gate"]
 
@@ -79,7 +81,7 @@ def _rows_view(t: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]
 
 class _RmsnormSiluGate(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, z, weight, eps):
+    def forward(ctx, x, z, weight, eps, keep):
         if not (x.is_cuda and z.is_cuda and weight.is_cuda):
             raise ValueError("rmsnorm_silu_gate: x, z and weight must be CUDA tensors")
         if x.shape != z.shape:
@@ -90,51 +92,67 @@ class _RmsnormSiluGate(torch.autograd.Function):
             raise ValueError(f"rmsnorm_silu_gate: weight must be [{HEAD_DIM}]; got {tuple(weight.shape)}")
         y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
         rows = x.numel() // HEAD_DIM
+        kept = ()
+        if keep:
+            codes = lambda *shape: torch.empty(shape, dtype=torch.uint8, device=x.device)  # noqa: E731
+            kept = (codes(rows, HEAD_DIM), codes(rows, HEAD_DIM), codes(rows),
+                    torch.empty(rows, dtype=torch.float32, device=x.device))
         if rows:
             xv, heads, xt, xh = _rows_view(x, "x")
             zv, z_heads, zt, zh = _rows_view(z, "z")
             if z_heads != heads:
                 raise ValueError("rmsnorm_silu_gate: x and z must split their rows into the same heads")
             with torch.cuda.device(x.device):
-                native.launch("gated_rmsnorm_fwd", xv, zv, weight.contiguous(), y, rows, heads, xt, xh, zt, zh,
-                              float(eps), device=x.device)
-        ctx.save_for_backward(x, z, weight)
-        ctx.eps = float(eps)
+                native.launch("gated_rmsnorm_fwd_keep" if keep else "gated_rmsnorm_fwd", xv, zv, weight.contiguous(), y,
+                              *kept, rows, heads, xt, xh, zt, zh, float(eps), device=x.device)
+        ctx.save_for_backward(*(kept or (x, z)), weight)
+        ctx.eps, ctx.keep, ctx.shape = float(eps), keep, x.shape
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, z, weight = ctx.saved_tensors
-        device = x.device
-        rows = x.numel() // HEAD_DIM
-        dx = torch.empty(x.shape, dtype=torch.bfloat16, device=device)
-        dz = torch.empty(x.shape, dtype=torch.bfloat16, device=device)
+        *kept, weight = ctx.saved_tensors
+        device = weight.device
+        rows = ctx.shape.numel() // HEAD_DIM
+        dx = torch.empty(ctx.shape, dtype=torch.bfloat16, device=device)
+        dz = torch.empty(ctx.shape, dtype=torch.bfloat16, device=device)
         want_dw = ctx.needs_input_grad[2]
         dw = torch.zeros(HEAD_DIM, dtype=torch.bfloat16, device=device) if want_dw else None
         if rows:
-            xv, heads, xt, xh = _rows_view(x, "x")
-            zv, _, zt, zh = _rows_view(z, "z")
             dy = dy.contiguous() if dy.dtype == torch.bfloat16 else dy.to(torch.bfloat16).contiguous()
             with torch.cuda.device(device):
                 partial = None
                 if want_dw:
                     blocks = native.library().mek_gated_rmsnorm_partial_rows(native.ctypes.c_int64(rows))
                     partial = workspace.take(OP, "dw_partial", (blocks, HEAD_DIM), torch.float32, device)
-                native.launch("gated_rmsnorm_bwd", dy, xv, zv, weight.contiguous(), dx, dz, partial, dw, rows, heads,
-                              xt, xh, zt, zh, ctx.eps, device=device)
-        return dx, dz, dw, None
+                if ctx.keep:
+                    native.launch("gated_rmsnorm_bwd_kept", dy, *kept, weight.contiguous(), dx, dz, partial, dw, rows,
+                                  device=device)
+                else:
+                    xv, heads, xt, xh = _rows_view(kept[0], "x")
+                    zv, _, zt, zh = _rows_view(kept[1], "z")
+                    native.launch("gated_rmsnorm_bwd", dy, xv, zv, weight.contiguous(), dx, dz, partial, dw, rows, heads,
+                                  xt, xh, zt, zh, ctx.eps, device=device)
+        return dx, dz, dw, None, None
 
 
-def rmsnorm_silu_gate(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6) -> torch.Tensor:
+def rmsnorm_silu_gate(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
+                      checkpoint: str | None = None) -> torch.Tensor:
     """Autograd-enabled ``RMSNorm(x) * weight * SiLU(z)`` over the last dimension (128).
 
     ``x`` and ``z``: BF16 of one ``[..., 128]`` shape; a gate that is a column slice of a wider projection is read in
     place when its last stride is 1, its token and head strides are multiples of 8 elements and it is 16-byte aligned,
     else copied once (the same bits either way).  ``weight``: BF16 ``[128]``.  Returns BF16 ``y`` of ``x``'s shape;
     every gradient comes in BF16 and the weight gradient sums over the rows of this call only (reference:
-    ops.py:126-148)."""
+    ops.py:126-148).
+
+    ``checkpoint`` (an extension of the reference's signature): ``None`` keeps ``x`` and ``z`` for the backward, ``"e4m3"``
+    keeps ``x * rstd`` and ``z`` in 8 bits, each off by at most 2^-4 of its value (an ``x * rstd`` below 2^-6 by at
+    most 2^-10; a ``z`` below 2^-13 of its row's largest by at most 2^-17 of that one; a ``z`` that is not finite is NaN to
+    the gradients).  ``y`` does not
+    change."""
     config.variant(OP)  # both variants run the same kernels; an unknown configuration still raises here
-    return _RmsnormSiluGate.apply(x, z, weight, eps)
+    return _RmsnormSiluGate.apply(x, z, weight, eps, checkpoint_format(OP, checkpoint))
 
 
 def prebuild(*, device: Any = None, max_workers: int | None = None) -> list[Path]:

@@ -9,7 +9,13 @@
 // row order (FP32), a block adds its 8 warps in warp order (FP32), and a second launch adds the blocks' partial sums
 // in block order in FP64.  The number of blocks is a function of the row count alone, so identical inputs give
 // identical bits.
+//
+// 8-bit checkpoint: the forward may also write what the backward needs as e4m3 codes -- the normalised row n = x rstd,
+// whose values stay below sqrt(128) and need no scale, and z under one power of two a row (exact to divide by, so
+// the code's rounding is the only error) -- and the backward read them in the place of x and z: 2 bytes an element kept
+// instead of 4.
 #include "common.cuh"
+#include "rowio.cuh"
 #include "umma.cuh"
 
 namespace mek {
@@ -41,9 +47,30 @@ __device__ __forceinline__ float half_warp_sum(float x) {
   return x;
 }
 
+__device__ __forceinline__ float half_warp_max(float x) {
+#pragma unroll
+  for (int m = 8; m >= 1; m >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
+  return x;
+}
+
+// The smallest e >= -126 with most <= 448 2^e, from the bits of most >= 0 (448 = 0.875 2^9).
+__device__ __forceinline__ int e4m3_exponent(float most) {
+  const int bits = __float_as_int(most);
+  return max((bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0), -126);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// A row of the checkpoint: codes of n and of z 2^-e, e (biased by 127), rstd.
+struct NormCheckpoint {
+  uint8_t *n_codes, *z_codes, *z_exponent;
+  float* rstd;
+};
+
+// kKeep: the checkpoint is written too; y does not depend on it.
+template <bool kKeep>
 __global__ void __launch_bounds__(256) gated_rmsnorm_fwd_kernel(RowView x, RowView z, const __nv_bfloat16* __restrict__ w,
                                                                 __nv_bfloat16* __restrict__ y, int64_t rows, int heads,
-                                                                float eps) {
+                                                                float eps, NormCheckpoint keep) {
   const int l16 = threadIdx.x & 15, half = threadIdx.x >> 4;  // 16 half-warps per block, 2 rows each
   const int64_t r0 = int64_t(blockIdx.x) * kNormRowsPerBlock + half * 2;
   float wv[8], xv[2][8], zv[2][8];
@@ -63,6 +90,82 @@ __global__ void __launch_bounds__(256) gated_rmsnorm_fwd_kernel(RowView x, RowVi
 #pragma unroll
     for (int j = 0; j < 8; ++j) out[j] = ((xv[i][j] * rstd) * wv[j]) * __fdividef(zv[i][j], 1.0f + __expf(-zv[i][j]));
     if (r0 + i < rows) store8(y + (r0 + i) * 128, l16, out);
+    if constexpr (kKeep) {
+      float most = 0.f, n[8], scaled[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = fmaxf(most, isfinite(zv[i][j]) ? fabsf(zv[i][j]) : 0.f);
+      const int e = e4m3_exponent(half_warp_max(most));
+      const float down = power_of_two(-e);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        n[j] = xv[i][j] * rstd;
+        scaled[j] = isfinite(zv[i][j]) ? zv[i][j] * down : __int_as_float(0x7fffffff);  // e4m3 has NaN, no infinity
+      }
+      if (r0 + i < rows) {
+        const int64_t r = r0 + i;
+        reinterpret_cast<Vec<uint8_t, 8>*>(keep.n_codes + r * 128)[l16] = to_e4m3(n);
+        reinterpret_cast<Vec<uint8_t, 8>*>(keep.z_codes + r * 128)[l16] = to_e4m3(scaled);
+        if (l16 == 0) keep.z_exponent[r] = uint8_t(e + 127), keep.rstd[r] = rstd;
+      }
+    }
+  }
+}
+
+// The backward from the checkpoint; formulas as below with n and z as the codes hold them.
+__global__ void __launch_bounds__(256) gated_rmsnorm_bwd_kept_kernel(const __nv_bfloat16* __restrict__ dy,
+                                                                     NormCheckpoint kept,
+                                                                     const __nv_bfloat16* __restrict__ w,
+                                                                     __nv_bfloat16* __restrict__ dx,
+                                                                     __nv_bfloat16* __restrict__ dz,
+                                                                     float* __restrict__ dw_partial, int64_t rows) {
+  __shared__ float s_dw[16][128];
+  const int l16 = threadIdx.x & 15, half = threadIdx.x >> 4;
+  float wv[8], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  load8(w, l16, wv);
+  for (int64_t group = blockIdx.x; group * kNormRowsPerBlock < rows; group += gridDim.x) {
+    const int64_t r0 = group * kNormRowsPerBlock + half * 2;
+    float n[2][8], zv[2][8], gv[2][8], rstd[2], up[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
+      from_e4m3(reinterpret_cast<const Vec<uint8_t, 8>*>(kept.n_codes + r * 128)[l16], n[i]);
+      from_e4m3(reinterpret_cast<const Vec<uint8_t, 8>*>(kept.z_codes + r * 128)[l16], zv[i]);
+      load8(dy + r * 128, l16, gv[i]);
+      rstd[i] = kept.rstd[r];
+      up[i] = power_of_two(int(kept.z_exponent[r]) - 127);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool live = r0 + i < rows;  // uniform over the half-warp
+      float dot = 0.f, dn[8], dzv[8], dxv[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float z = zv[i][j] * up[i];
+        const float s = __fdividef(1.0f, 1.0f + __expf(-z));
+        const float a = gv[i][j] * (z * s);
+        dn[j] = a * wv[j];
+        dot = fmaf(dn[j], n[i][j], dot);
+        dzv[j] = gv[i][j] * n[i][j] * wv[j] * s * (1.0f + z * (1.0f - s));
+        if (live) acc[j] = fmaf(a, n[i][j], acc[j]);
+      }
+      const float mean = half_warp_sum(dot) * (1.0f / 128.0f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dxv[j] = rstd[i] * (dn[j] - n[i][j] * mean);
+      if (live) {
+        store8(dx + (r0 + i) * 128, l16, dxv);
+        store8(dz + (r0 + i) * 128, l16, dzv);
+      }
+    }
+  }
+  if (dw_partial == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s_dw[half][l16 * 8 + j] = acc[j];
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    float sum = 0.f;
+#pragma unroll
+    for (int hw = 0; hw < 16; ++hw) sum += s_dw[hw][threadIdx.x];
+    dw_partial[int64_t(blockIdx.x) * 128 + threadIdx.x] = sum;
   }
 }
 
@@ -156,6 +259,32 @@ int check_norm(const char* what, int64_t rows, int heads, int64_t xt, int64_t xh
   return MEK_OK;
 }
 
+int check_checkpoint(const char* what, const mek::NormCheckpoint& c) {
+  using namespace mek;
+  if (!c.n_codes || !c.z_codes || !c.z_exponent || !c.rstd) return fail(MEK_ERR_INVALID, "%s: a null pointer", what);
+  if ((reinterpret_cast<uintptr_t>(c.n_codes) | reinterpret_cast<uintptr_t>(c.z_codes)) % 8 != 0)
+    return fail(MEK_ERR_INVALID, "%s: the codes must be 8-byte aligned", what);
+  return MEK_OK;
+}
+
+int norm_fwd(const char* what, const void* x, const void* z, const void* weight, void* y,
+             const mek::NormCheckpoint* keep, int64_t rows, int heads, int64_t x_token_stride, int64_t x_head_stride,
+             int64_t z_token_stride, int64_t z_head_stride, float eps, void* stream) {
+  using namespace mek;
+  if (!x || !z || !weight || !y) return fail(MEK_ERR_INVALID, "%s: a null pointer", what);
+  if (int rc = check_norm(what, rows, heads, x_token_stride, x_head_stride, z_token_stride, z_head_stride, x, z))
+    return rc;
+  const RowView xv{static_cast<const __nv_bfloat16*>(x), x_token_stride, x_head_stride};
+  const RowView zv{static_cast<const __nv_bfloat16*>(z), z_token_stride, z_head_stride};
+  const unsigned grid = unsigned((rows + kNormRowsPerBlock - 1) / kNormRowsPerBlock);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const __nv_bfloat16* w = static_cast<const __nv_bfloat16*>(weight);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(y);
+  if (keep) gated_rmsnorm_fwd_kernel<true><<<grid, 256, 0, s>>>(xv, zv, w, out, rows, heads, eps, *keep);
+  else gated_rmsnorm_fwd_kernel<false><<<grid, 256, 0, s>>>(xv, zv, w, out, rows, heads, eps, NormCheckpoint{});
+  return launched(what);
+}
+
 }  // namespace
 
 extern "C" {
@@ -165,17 +294,43 @@ int mek_gated_rmsnorm_partial_rows(int64_t rows) { return rows > 0 ? norm_blocks
 int mek_gated_rmsnorm_fwd(const void* x, const void* z, const void* weight, void* y, int64_t rows, int heads,
                           int64_t x_token_stride, int64_t x_head_stride, int64_t z_token_stride, int64_t z_head_stride,
                           float eps, void* stream) {
+  return norm_fwd("gated_rmsnorm_fwd", x, z, weight, y, nullptr, rows, heads, x_token_stride, x_head_stride,
+                  z_token_stride, z_head_stride, eps, stream);
+}
+
+int mek_gated_rmsnorm_fwd_keep(const void* x, const void* z, const void* weight, void* y, uint8_t* n_codes,
+                               uint8_t* z_codes, uint8_t* z_exponent, float* rstd, int64_t rows, int heads,
+                               int64_t x_token_stride, int64_t x_head_stride, int64_t z_token_stride,
+                               int64_t z_head_stride, float eps, void* stream) {
+  const mek::NormCheckpoint keep{n_codes, z_codes, z_exponent, rstd};
+  if (int rc = check_checkpoint("gated_rmsnorm_fwd_keep", keep)) return rc;
+  return norm_fwd("gated_rmsnorm_fwd_keep", x, z, weight, y, &keep, rows, heads, x_token_stride, x_head_stride,
+                  z_token_stride, z_head_stride, eps, stream);
+}
+
+int mek_gated_rmsnorm_bwd_kept(const void* dy, const uint8_t* n_codes, const uint8_t* z_codes,
+                               const uint8_t* z_exponent, const float* rstd, const void* weight, void* dx, void* dz,
+                               float* dw_partial, void* dw, int64_t rows, void* stream) {
   using namespace mek;
-  if (!x || !z || !weight || !y) return fail(MEK_ERR_INVALID, "gated_rmsnorm_fwd: a null pointer");
-  if (int rc = check_norm("gated_rmsnorm_fwd", rows, heads, x_token_stride, x_head_stride, z_token_stride,
-                          z_head_stride, x, z))
-    return rc;
-  const RowView xv{static_cast<const __nv_bfloat16*>(x), x_token_stride, x_head_stride};
-  const RowView zv{static_cast<const __nv_bfloat16*>(z), z_token_stride, z_head_stride};
-  const unsigned grid = unsigned((rows + kNormRowsPerBlock - 1) / kNormRowsPerBlock);
-  gated_rmsnorm_fwd_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      xv, zv, static_cast<const __nv_bfloat16*>(weight), static_cast<__nv_bfloat16*>(y), rows, heads, eps);
-  return launched("gated_rmsnorm_fwd");
+  if (!dy || !weight || !dx || !dz) return fail(MEK_ERR_INVALID, "gated_rmsnorm_bwd_kept: a null pointer");
+  const NormCheckpoint kept{const_cast<uint8_t*>(n_codes), const_cast<uint8_t*>(z_codes),
+                            const_cast<uint8_t*>(z_exponent), const_cast<float*>(rstd)};
+  if (int rc = check_checkpoint("gated_rmsnorm_bwd_kept", kept)) return rc;
+  if ((dw == nullptr) != (dw_partial == nullptr))
+    return fail(MEK_ERR_INVALID, "gated_rmsnorm_bwd_kept: dw and its partial sums go together");
+  if (rows <= 0) return fail(MEK_ERR_INVALID, "gated_rmsnorm_bwd_kept: rows=%lld must be positive", (long long)rows);
+  const int blocks = norm_blocks(rows);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  gated_rmsnorm_bwd_kept_kernel<<<blocks, 256, 0, s>>>(static_cast<const __nv_bfloat16*>(dy), kept,
+                                                       static_cast<const __nv_bfloat16*>(weight),
+                                                       static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dz),
+                                                       dw_partial, rows);
+  if (int rc = launched("gated_rmsnorm_bwd_kept")) return rc;
+  if (dw != nullptr) {
+    gated_rmsnorm_dw_kernel<<<1, 128, 0, s>>>(dw_partial, blocks, static_cast<__nv_bfloat16*>(dw));
+    return launched("gated_rmsnorm_bwd_kept (weight gradient)");
+  }
+  return MEK_OK;
 }
 
 int mek_gated_rmsnorm_bwd(const void* dy, const void* x, const void* z, const void* weight, void* dx, void* dz,
