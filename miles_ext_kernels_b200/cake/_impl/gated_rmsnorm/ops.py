@@ -22,12 +22,17 @@ import torch
 
 from ..._runtime import config, loader, registry, workspace
 from ..gdn import native
-from ..rows import checkpoint_format
+from ..gdn.native import pointer
+from ..rows import checkpoint_format, on_device
 
 __all__ = ["check_supported", "prebuild", "release", "rmsnorm_silu_gate"]
 
 OP = "gated_rmsnorm"
 HEAD_DIM = 128
+_fwd = native.Entry("gated_rmsnorm_fwd", "pppplillllf")
+_fwd_keep = native.Entry("gated_rmsnorm_fwd_keep", "pppppppplillllf")
+_bwd = native.Entry("gated_rmsnorm_bwd", "pppppppplillllf")
+_bwd_kept = native.Entry("gated_rmsnorm_bwd_kept", "ppppppppppl")
 _BACKEND = "--linear-attention-output-norm-backend cake"
 
 
@@ -90,49 +95,52 @@ class _RmsnormSiluGate(torch.autograd.Function):
             raise NotImplementedError("rmsnorm_silu_gate: x, z and weight must be bfloat16")
         if tuple(weight.shape) != (HEAD_DIM,):
             raise ValueError(f"rmsnorm_silu_gate: weight must be [{HEAD_DIM}]; got {tuple(weight.shape)}")
-        y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        device = x.device
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
         rows = x.numel() // HEAD_DIM
         kept = ()
         if keep:
-            codes = lambda *shape: torch.empty(shape, dtype=torch.uint8, device=x.device)  # noqa: E731
-            kept = (codes(rows, HEAD_DIM), codes(rows, HEAD_DIM), codes(rows),
-                    torch.empty(rows, dtype=torch.float32, device=x.device))
+            kept = (x.new_empty((rows, HEAD_DIM), dtype=torch.uint8), x.new_empty((rows, HEAD_DIM), dtype=torch.uint8),
+                    x.new_empty(rows, dtype=torch.uint8), x.new_empty(rows, dtype=torch.float32))
         if rows:
             xv, heads, xt, xh = _rows_view(x, "x")
             zv, z_heads, zt, zh = _rows_view(z, "z")
             if z_heads != heads:
                 raise ValueError("rmsnorm_silu_gate: x and z must split their rows into the same heads")
-            with torch.cuda.device(x.device):
-                native.launch("gated_rmsnorm_fwd_keep" if keep else "gated_rmsnorm_fwd", xv, zv, weight.contiguous(), y,
-                              *kept, rows, heads, xt, xh, zt, zh, float(eps), device=x.device)
+            w = weight.contiguous()
+            with on_device(device):
+                (_fwd_keep if keep else _fwd)(device, xv.data_ptr(), zv.data_ptr(), w.data_ptr(), y.data_ptr(),
+                                              *(t.data_ptr() for t in kept), rows, heads, xt, xh, zt, zh, float(eps))
         ctx.save_for_backward(*(kept or (x, z)), weight)
-        ctx.eps, ctx.keep, ctx.shape = float(eps), keep, x.shape
+        ctx.eps, ctx.keep = float(eps), keep
         return y
 
     @staticmethod
     def backward(ctx, dy):
         *kept, weight = ctx.saved_tensors
-        device = weight.device
-        rows = ctx.shape.numel() // HEAD_DIM
-        dx = torch.empty(ctx.shape, dtype=torch.bfloat16, device=device)
-        dz = torch.empty(ctx.shape, dtype=torch.bfloat16, device=device)
+        device = dy.device
+        rows = dy.numel() // HEAD_DIM
+        dy = dy.contiguous() if dy.dtype == torch.bfloat16 else dy.to(torch.bfloat16).contiguous()
+        dx, dz = torch.empty_like(dy), torch.empty_like(dy)
         want_dw = ctx.needs_input_grad[2]
-        dw = torch.zeros(HEAD_DIM, dtype=torch.bfloat16, device=device) if want_dw else None
+        dw = weight.new_empty(HEAD_DIM) if want_dw else None
+        if not rows and want_dw:
+            dw.zero_()
         if rows:
-            dy = dy.contiguous() if dy.dtype == torch.bfloat16 else dy.to(torch.bfloat16).contiguous()
-            with torch.cuda.device(device):
+            w = weight.contiguous()
+            with on_device(device):
                 partial = None
                 if want_dw:
                     blocks = native.library().mek_gated_rmsnorm_partial_rows(native.ctypes.c_int64(rows))
                     partial = workspace.take(OP, "dw_partial", (blocks, HEAD_DIM), torch.float32, device)
                 if ctx.keep:
-                    native.launch("gated_rmsnorm_bwd_kept", dy, *kept, weight.contiguous(), dx, dz, partial, dw, rows,
-                                  device=device)
+                    _bwd_kept(device, dy.data_ptr(), *(t.data_ptr() for t in kept), w.data_ptr(), dx.data_ptr(),
+                              dz.data_ptr(), pointer(partial), pointer(dw), rows)
                 else:
                     xv, heads, xt, xh = _rows_view(kept[0], "x")
                     zv, _, zt, zh = _rows_view(kept[1], "z")
-                    native.launch("gated_rmsnorm_bwd", dy, xv, zv, weight.contiguous(), dx, dz, partial, dw, rows, heads,
-                                  xt, xh, zt, zh, ctx.eps, device=device)
+                    _bwd(device, dy.data_ptr(), xv.data_ptr(), zv.data_ptr(), w.data_ptr(), dx.data_ptr(), dz.data_ptr(),
+                         pointer(partial), pointer(dw), rows, heads, xt, xh, zt, zh, ctx.eps)
         return dx, dz, dw, None, None
 
 

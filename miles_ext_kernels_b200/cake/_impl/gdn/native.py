@@ -16,7 +16,7 @@ import torch
 
 from ..._runtime import loader
 
-__all__ = ["Dims", "LaunchLog", "library", "launch", "release", "set_launch_log"]
+__all__ = ["Dims", "Entry", "LaunchLog", "library", "launch", "pointer", "release", "set_launch_log"]
 
 
 class Dims(ctypes.Structure):
@@ -110,6 +110,48 @@ def launch(name: str, *arguments: Any, device: torch.device | None = None) -> No
         end.record(current)
         log.events.append((name, start, end))
     lib.check(code)
+
+
+def pointer(tensor: torch.Tensor | None) -> int | None:
+    """The device pointer an :class:`Entry` takes for a tensor or for an absent one."""
+    return None if tensor is None else tensor.data_ptr()
+
+
+_KINDS = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_int64, "f": ctypes.c_float}
+
+
+class Entry:
+    """One entry point with its prototype bound once: ``Entry("layer_norm_fwd", "pip...")(device, *arguments)`` is
+    ``launch`` without its cost per argument (a letter each: ``p`` pointer, ``i`` int, ``l`` int64, ``f`` float; the
+    stream follows by itself).  For the ops whose small calls are bound by the host."""
+
+    __slots__ = ("_call", "_name", "_owner", "_types")
+
+    def __init__(self, name: str, kinds: str) -> None:
+        self._name = name
+        self._types = tuple(_KINDS[kind] for kind in kinds) + (ctypes.c_void_p,)
+        self._owner = self._call = None
+
+    def __call__(self, device: torch.device, *arguments: Any) -> None:
+        lib = _library
+        if lib is None or lib is not self._owner:
+            lib = self._owner = library()
+            self._call = ctypes.CFUNCTYPE(ctypes.c_int, *self._types)((f"mek_{self._name}", lib._dll))
+        index = device.index
+        stream = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
+        log = _log
+        if log is not None:
+            log.count += 1
+            if log.timed:
+                current = torch.cuda.current_stream(device)
+                start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+                start.record(current)
+        code = self._call(*arguments, stream)
+        if log is not None and log.timed:
+            end.record(current)
+            log.events.append((self._name, start, end))
+        if code:
+            lib.check(code)
 
 
 def release() -> None:

@@ -16,19 +16,22 @@ parameter gradients are summed in FP32 per block and in FP64 across the blocks, 
 
 from __future__ import annotations
 
+from ctypes import c_int64
 from pathlib import Path
 from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ..._runtime import config, loader, registry, workspace
+from ..._runtime import loader, registry, workspace
 from ..gdn import native
-from ..rows import TYPES, check_device, checkpoint_format, on_device
+from ..gdn.native import pointer
+from ..rows import TYPES, check_device, checkpoint_format, on_device, once_differentiable
 
 __all__ = ["check_supported", "layer_norm", "prebuild", "release"]
 
 OP = "layer_norm"
+_fwd = native.Entry("layer_norm_fwd", "pippipppplllf")
+_bwd = native.Entry("layer_norm_bwd", "ppippppipppplll")
 _CHECKPOINT_WIDTH = 200704  # 448^2: a wider row's largest value could exceed e4m3
 
 
@@ -69,64 +72,68 @@ def _rows_of(x: torch.Tensor) -> torch.Tensor:
 
 
 def _forward(x, weight, bias, eps, keep, train):
-    """``(y, kept)``: ``kept`` is what the backward reads -- ``(x, None, mean, rstd)`` or ``(None, codes, None, rstd)``,
-    ``None`` when there will be none."""
+    """``(y, kept)``: ``kept`` is what the backward reads -- ``(x, None, statistics)`` or ``(None, codes, statistics)``
+    with the statistics ``[mean, rstd]`` or ``[rstd]`` of the rows, ``None`` when there will be none."""
     width = x.shape[-1]
-    device = x.device
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     rows = x.numel() // width
-    mean = rstd = codes = None
+    mean = rstd = codes = statistics = None
     if train:
-        rstd = torch.empty(rows, dtype=torch.float32, device=device)
+        statistics = x.new_empty((1 if keep else 2, rows), dtype=torch.float32)
+        rstd = statistics.data_ptr() + (0 if keep else 4 * rows)
         if keep:
-            codes = torch.empty((rows, width), dtype=torch.uint8, device=device)
+            codes = x.new_empty((rows, width), dtype=torch.uint8)
         else:
-            mean = torch.empty(rows, dtype=torch.float32, device=device)
+            mean = statistics.data_ptr()
     if rows:
         xv = _rows_of(x)
         param = weight if weight is not None else bias
-        with on_device(device):
-            native.launch("layer_norm_fwd", xv, TYPES[x.dtype], weight, bias, TYPES[param.dtype] if param is not None else 0,
-                          y, mean, rstd, codes, rows, width, xv.stride(0), eps, device=device)
-    return y, ((None if keep else x), codes, mean, rstd) if train else None
+        with on_device(x.device):
+            _fwd(x.device, xv.data_ptr(), TYPES[x.dtype], pointer(weight), pointer(bias),
+                 TYPES[param.dtype] if param is not None else 0, y.data_ptr(), mean, rstd, pointer(codes), rows, width,
+                 xv.stride(0), eps)
+    return y, ((None if keep else x), codes, statistics) if train else None
+
+
+def _gradients(ctx, dy):
+    x, codes, statistics, weight, bias = ctx.saved_tensors
+    device = dy.device
+    width = ctx.shape[-1]
+    rows = statistics.shape[1]
+    dy = dy.contiguous()
+    dx = torch.empty_like(dy)
+    _, want_dw, want_db, _, _ = ctx.needs_input_grad
+    dw = torch.empty_like(weight) if want_dw else None
+    db = torch.empty_like(bias) if want_db else None
+    if not rows:
+        for grad in (dw, db):
+            if grad is not None:
+                grad.zero_()
+        return dx, dw, db, None, None
+    xv = None if x is None else _rows_of(x)
+    kind = TYPES[dy.dtype]
+    param = weight if weight is not None else bias
+    with on_device(device):
+        partial = None
+        if want_dw or want_db:
+            blocks = native.library().mek_layer_norm_partial_rows(c_int64(rows), c_int64(width), kind)
+            partial = workspace.take(OP, "partial", (blocks, 2, width), torch.float32, device)
+        first = statistics.data_ptr()
+        _bwd(device, dy.data_ptr(), pointer(xv), kind, pointer(codes), None if x is None else first,
+             first if x is None else first + 4 * rows, pointer(weight), TYPES[param.dtype] if param is not None else 0,
+             dx.data_ptr(), pointer(partial), pointer(dw), pointer(db), rows, width, 0 if xv is None else xv.stride(0))
+    return dx, dw, db, None, None
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
         y, kept = _forward(x, weight, bias, eps, keep, True)
-        ctx.save_for_backward(*kept, weight)
-        ctx.shape, ctx.dtype, ctx.bias_dtype = x.shape, x.dtype, None if bias is None else bias.dtype
+        ctx.save_for_backward(*kept, weight, bias)
+        ctx.shape = x.shape
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, codes, mean, rstd, weight = ctx.saved_tensors
-        device = dy.device
-        width = ctx.shape[-1]
-        rows = rstd.shape[0]
-        dy = dy.contiguous()
-        dx = torch.empty(ctx.shape, dtype=ctx.dtype, device=device)
-        param_dtype = weight.dtype if weight is not None else ctx.bias_dtype
-        dw = torch.empty(width, dtype=param_dtype, device=device) if ctx.needs_input_grad[1] else None
-        db = torch.empty(width, dtype=param_dtype, device=device) if ctx.needs_input_grad[2] else None
-        if not rows:
-            for grad in (dw, db):
-                if grad is not None:
-                    grad.zero_()
-            return dx, dw, db, None, None
-        xv = None if x is None else _rows_of(x)
-        with on_device(device):
-            partial = None
-            if dw is not None or db is not None:
-                blocks = native.library().mek_layer_norm_partial_rows(
-                    native.ctypes.c_int64(rows), native.ctypes.c_int64(width), TYPES[ctx.dtype])
-                partial = workspace.take(OP, "partial", (blocks, 2, width), torch.float32, device)
-            native.launch("layer_norm_bwd", dy, xv, TYPES[ctx.dtype], codes, mean, rstd, weight,
-                          TYPES[param_dtype] if param_dtype is not None else 0, dx, partial, dw, db, rows, width,
-                          0 if xv is None else xv.stride(0), device=device)
-        return dx, dw, db, None, None
+    backward = staticmethod(once_differentiable(_gradients))
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, *,
@@ -137,7 +144,6 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     them, else copied once (the same bits either way).  ``weight``, ``bias``: ``[C]``, each optional, both of one type
     out of the three, which their gradients have too.  ``checkpoint``: ``None`` keeps ``x`` for the backward, ``"e4m3"``
     keeps the normalised rows in 8 bits instead (``C`` up to 200,704).  Not twice differentiable."""
-    config.variant(OP)  # both variants run the same kernels; an unknown configuration still raises here
     keep = checkpoint_format(OP, checkpoint)
     if x.dim() < 1:
         raise ValueError("layer_norm: x must have at least one dimension")

@@ -16,15 +16,18 @@ from pathlib import Path
 from typing import Any
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from ..._runtime import config, loader, registry, workspace
+from ..._runtime import loader, registry, workspace
 from ..gdn import native
-from ..rows import TYPES, check_device, on_device
+from ..gdn.native import pointer
+from ..rows import TYPES, check_device, on_device, once_differentiable
 
 __all__ = ["check_supported", "gated_linear_recurrence", "gated_linear_recurrence_step", "prebuild", "release"]
 
 OP = "linear_recurrence"
+_fwd = native.Entry("linear_recurrence_fwd", "pipiplllllllplpppp")
+_bwd = native.Entry("linear_recurrence_bwd", "ppipipplllllllplppppp")
+_step = native.Entry("linear_recurrence_step", "pipippipllllll")
 _MAX_TOKENS, _MAX_CHANNELS = 1 << 30, 1 << 23
 
 
@@ -60,6 +63,15 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _flat_rows(t: torch.Tensor, channels: int) -> torch.Tensor:
+    """``t [R, ...]`` as ``[R, C]`` with unit stride over the channels, in place where it can be, else copied once."""
+    if t.dim() != 2:
+        t = t.reshape(t.shape[0], channels)  # a view where the trailing dimensions merge
+    if t.stride(1) != 1 and channels > 1:
+        t = t.contiguous()
+    return t
+
+
 def _tiles(tokens: int) -> int:
     return -(-tokens // native.library().mek_linear_recurrence_tile())
 
@@ -69,21 +81,41 @@ def _forward(x, g, h0, cu, want_final, train):
     batch, tokens, channels = x.shape
     device = x.device
     sequences = batch if cu is None else cu.numel() - 1
-    y = torch.empty((batch, tokens, channels), dtype=x.dtype, device=device)
-    final = torch.empty((sequences, channels), dtype=torch.float32, device=device) if want_final else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    final = x.new_empty((sequences, channels), dtype=torch.float32) if want_final else None
     with on_device(device):
         tiles = _tiles(tokens)
         scratch = ends = None
         if tiles > 1:
             scratch = workspace.take(OP, "scratch", (2, batch, tiles, channels), torch.float32, device)
             if train:
-                ends = torch.empty((batch, tiles, channels), dtype=torch.float32, device=device)
+                ends = x.new_empty((batch, tiles, channels), dtype=torch.float32)
             else:
                 ends = workspace.take(OP, "ends", (batch, tiles, channels), torch.float32, device)
-        native.launch("linear_recurrence_fwd", x, TYPES[x.dtype], g, TYPES[g.dtype], y, batch, tokens, channels,
-                      x.stride(0), x.stride(1), g.stride(0), g.stride(1), cu, sequences, h0, final, scratch, ends,
-                      device=device)
+        _fwd(device, x.data_ptr(), TYPES[x.dtype], g.data_ptr(), TYPES[g.dtype], y.data_ptr(), batch, tokens, channels,
+             *x.stride()[:2], *g.stride()[:2], pointer(cu), sequences, pointer(h0), pointer(final), pointer(scratch),
+             pointer(ends))
     return y, final, ends
+
+
+def _gradients(ctx, dy, d_final):
+    x, g, h0, cu, ends = ctx.saved_tensors
+    batch, tokens, channels = x.shape
+    device = x.device
+    sequences = batch if cu is None else cu.numel() - 1
+    dy = dy.contiguous()
+    d_final = None if d_final is None else d_final.contiguous()
+    dx = torch.empty_like(dy)
+    dg = torch.empty_like(g, memory_format=torch.contiguous_format)
+    dh0 = torch.empty_like(h0) if ctx.needs_input_grad[2] else None
+    with on_device(device):
+        scratch = None
+        if ends is not None:
+            scratch = workspace.take(OP, "scratch", (3, *ends.shape), torch.float32, device)
+        _bwd(device, dy.data_ptr(), x.data_ptr(), TYPES[x.dtype], g.data_ptr(), TYPES[g.dtype], dx.data_ptr(),
+             dg.data_ptr(), batch, tokens, channels, *x.stride()[:2], *g.stride()[:2], pointer(cu), sequences,
+             pointer(h0), pointer(d_final), pointer(ends), pointer(dh0), pointer(scratch))
+    return dx, dg, dh0, None, None
 
 
 class _GatedLinearRecurrence(torch.autograd.Function):
@@ -93,26 +125,7 @@ class _GatedLinearRecurrence(torch.autograd.Function):
         ctx.save_for_backward(x, g, h0, cu, ends)
         return y, final
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, d_final):
-        x, g, h0, cu, ends = ctx.saved_tensors
-        batch, tokens, channels = x.shape
-        device = x.device
-        sequences = batch if cu is None else cu.numel() - 1
-        dy = dy.contiguous()
-        d_final = None if d_final is None else d_final.contiguous()
-        dx = torch.empty((batch, tokens, channels), dtype=x.dtype, device=device)
-        dg = torch.empty((batch, tokens, channels), dtype=g.dtype, device=device)
-        dh0 = torch.empty((sequences, channels), dtype=torch.float32, device=device) if ctx.needs_input_grad[2] else None
-        with on_device(device):
-            scratch = None
-            if ends is not None:
-                scratch = workspace.take(OP, "scratch", (3, *ends.shape), torch.float32, device)
-            native.launch("linear_recurrence_bwd", dy, x, TYPES[x.dtype], g, TYPES[g.dtype], dx, dg, batch, tokens, channels,
-                          x.stride(0), x.stride(1), g.stride(0), g.stride(1), cu, sequences, h0, d_final, ends, dh0,
-                          scratch, device=device)
-        return dx, dg, dh0, None, None
+    backward = staticmethod(once_differentiable(_gradients))
 
 
 def _no_tokens(x, g, h0, sequences, channels, want_final):
@@ -141,7 +154,6 @@ def gated_linear_recurrence(
     A sequence may be empty: its state passes through.  Tokens behind the last sequence belong to none: their ``y`` and
     gradients are zero.  ``final_state``: FP32 ``[N, ...]`` when ``output_final_state``, else ``None``.  Not twice
     differentiable."""
-    config.variant(OP)  # both variants run the same kernels; an unknown configuration still raises here
     if x.dim() < 3:
         raise ValueError(f"linear_recurrence: x must be [B, T, ...channels]; got {tuple(x.shape)}")
     if g.shape != x.shape:
@@ -195,7 +207,6 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
     autograd.  ``state_indices``: int32 or int64 ``[R]``, the slot of every row (``None``: row ``r`` uses slot ``r`` and
     ``N >= R``).  A row whose index is outside ``[0, N)``, -1 for example, is padding: no state changes and its ``y`` is
     zero.  Rows that name one slot are applied one after the other, in row order."""
-    config.variant(OP)
     if x.dim() < 2:
         raise ValueError(f"linear_recurrence: x must be [rows, ...channels]; got {tuple(x.shape)}")
     if g.shape != x.shape:
@@ -224,21 +235,24 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
             raise ValueError(f"linear_recurrence: {name} is on {t.device}, x on {x.device}")
     if not x.is_cuda:
         raise ValueError("linear_recurrence: x must be a CUDA tensor")
-    try:
-        pooled = state.view(pool, channels)
-    except RuntimeError:
-        pooled = None
+    pooled = state
+    if len(trailing) > 1:
+        try:
+            pooled = state.view(pool, channels)
+        except RuntimeError:
+            pooled = None
     if pooled is None or (channels > 1 and pooled.stride(1) != 1) or (pool > 1 and pooled.stride(0) < channels):
         raise ValueError(f"linear_recurrence: a state must be dense inside its slot; strides {state.stride()}")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     if rows == 0:
         return y
-    xv, gv = _rows(x[None])[0], _rows(g[None])[0]
+    xv, gv = _flat_rows(x, channels), _flat_rows(g, channels)
     slots = None if state_indices is None else state_indices.contiguous()
-    with on_device(x.device):
-        native.launch("linear_recurrence_step", xv, TYPES[x.dtype], gv, TYPES[g.dtype], pooled, slots,
-                      int(slots is not None and slots.dtype == torch.int64), y, rows, pool, channels, xv.stride(0),
-                      gv.stride(0), pooled.stride(0), device=x.device)
+    device = x.device
+    with on_device(device):
+        _step(device, xv.data_ptr(), TYPES[x.dtype], gv.data_ptr(), TYPES[g.dtype], pooled.data_ptr(), pointer(slots),
+              slots is not None and slots.dtype == torch.int64, y.data_ptr(), rows, pool, channels, xv.stride(0),
+              gv.stride(0), pooled.stride(0))
     return y
 
 

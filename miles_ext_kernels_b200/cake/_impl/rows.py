@@ -7,10 +7,11 @@ from contextlib import nullcontext
 from typing import Any
 
 import torch
+from torch.autograd.function import once_differentiable as _guarded
 
 from .._runtime import loader
 
-__all__ = ["CHECKPOINTS", "TYPES", "check_device", "checkpoint_format", "on_device"]
+__all__ = ["CHECKPOINTS", "TYPES", "check_device", "checkpoint_format", "on_device", "once_differentiable"]
 
 # element types of the C ABI
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -25,6 +26,17 @@ def on_device(device: torch.device) -> Any:
     if device.index is None or device.index == torch.cuda.current_device():
         return _NOTHING
     return torch.cuda.device(device)
+
+
+def once_differentiable(backward: Any) -> Any:
+    """``torch.autograd.function.once_differentiable``, which costs as much as a small backward's launch, where it can
+    matter: a backward that is itself being recorded (``create_graph=True``)."""
+    guarded = _guarded(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
 
 
 def checkpoint_format(op: str, checkpoint: Any) -> bool:
