@@ -345,9 +345,10 @@ int mek_layer_norm_bwd(const void* dy, const void* x, int type, const uint8_t* c
  * [num_seqs + 1] on the device, batch = 1) the tokens are packed sequences; y, dx, dg of tokens outside
  * [cu_seqlens[0], cu_seqlens[num_seqs]) are zero.  States fp32 [sequences, channels], each optional: initial_state
  * (NULL: zero), final_state, d_final_state (NULL: zero), dh0; a sequence without tokens passes its state through.
- * More than mek_linear_recurrence_tile() tokens need scratch fp32 [2, batch, tiles, channels] (backward: [3, ...])
- * with tiles = ceil(tokens / tile) and ends fp32 [batch, tiles, channels], the state after every tile, which the
- * backward reads.  step: one token of every row on a pool of states fp32 [pool, channels] (state_row_stride elements
+ * More than mek_linear_recurrence_tile() tokens need states fp32 [2 batch tiles channels + 1], 16-byte aligned, with
+ * tiles = ceil(tokens / tile): the state after every tile, which the backward reads; the backward needs scratch of the
+ * same size.  Blocks of one launch wait for one another through them (in an order that cannot block, and for at most
+ * a second: then the carried state is NaN), so no two calls that overlap may share them.  step: one token of every row on a pool of states fp32 [pool, channels] (state_row_stride elements
  * between them), updated in place: row r uses state slots[r] (int32, or int64 when slots_are_int64; NULL: r); a slot
  * outside [0, pool) leaves every state alone and gives zeros; rows that name one slot take their turns in row order.
  * No counterpart in the reference. */
@@ -355,13 +356,12 @@ int mek_linear_recurrence_tile(void);
 int mek_linear_recurrence_fwd(const void* x, int x_type, const void* g, int g_type, void* y, int64_t batch,
                               int64_t tokens, int64_t channels, int64_t x_batch_stride, int64_t x_token_stride,
                               int64_t g_batch_stride, int64_t g_token_stride, const int32_t* cu_seqlens, int64_t num_seqs,
-                              const float* initial_state, float* final_state, float* scratch, float* ends,
-                              void* stream);
+                              const float* initial_state, float* final_state, float* states, void* stream);
 int mek_linear_recurrence_bwd(const void* dy, const void* x, int x_type, const void* g, int g_type, void* dx, void* dg,
                               int64_t batch, int64_t tokens, int64_t channels, int64_t x_batch_stride,
                               int64_t x_token_stride, int64_t g_batch_stride, int64_t g_token_stride,
                               const int32_t* cu_seqlens, int64_t num_seqs, const float* initial_state,
-                              const float* d_final_state, const float* ends, float* dh0, float* scratch, void* stream);
+                              const float* d_final_state, const float* states, float* dh0, float* scratch, void* stream);
 int mek_linear_recurrence_step(const void* x, int x_type, const void* g, int g_type, float* state, const void* slots,
                                int slots_are_int64, void* y, int64_t rows, int64_t pool, int64_t channels,
                                int64_t x_row_stride, int64_t g_row_stride, int64_t state_row_stride, void* stream);

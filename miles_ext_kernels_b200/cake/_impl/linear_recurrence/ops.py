@@ -25,7 +25,7 @@ from ..rows import TYPES, check_device, on_device, once_differentiable
 __all__ = ["check_supported", "gated_linear_recurrence", "gated_linear_recurrence_step", "prebuild", "release"]
 
 OP = "linear_recurrence"
-_fwd = native.Entry("linear_recurrence_fwd", "pipiplllllllplpppp")
+_fwd = native.Entry("linear_recurrence_fwd", "pipiplllllllplppp")
 _bwd = native.Entry("linear_recurrence_bwd", "ppipipplllllllplppppp")
 _step = native.Entry("linear_recurrence_step", "pipippipllllll")
 _MAX_TOKENS, _MAX_CHANNELS = 1 << 30, 1 << 23
@@ -72,34 +72,33 @@ def _flat_rows(t: torch.Tensor, channels: int) -> torch.Tensor:
     return t
 
 
-def _tiles(tokens: int) -> int:
-    return -(-tokens // native.library().mek_linear_recurrence_tile())
+def _words(batch: int, tokens: int, channels: int) -> int:
+    """How many floats carry the state from tile to tile: 0 where one tile holds all tokens."""
+    tile = native.library().mek_linear_recurrence_tile()
+    return 2 * batch * -(-tokens // tile) * channels + 1 if tokens > tile else 0
 
 
 def _forward(x, g, h0, cu, want_final, train):
-    """``(y, final, ends)`` for ``x``, ``g [B, T, C]``; ``ends`` is ``None`` where one tile holds all tokens."""
+    """``(y, final, states)`` for ``x``, ``g [B, T, C]``; ``states`` holds the state after every tile for the backward
+    (``None`` where one tile holds all tokens)."""
     batch, tokens, channels = x.shape
     device = x.device
     sequences = batch if cu is None else cu.numel() - 1
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     final = x.new_empty((sequences, channels), dtype=torch.float32) if want_final else None
     with on_device(device):
-        tiles = _tiles(tokens)
-        scratch = ends = None
-        if tiles > 1:
-            scratch = workspace.take(OP, "scratch", (2, batch, tiles, channels), torch.float32, device)
-            if train:
-                ends = x.new_empty((batch, tiles, channels), dtype=torch.float32)
-            else:
-                ends = workspace.take(OP, "ends", (batch, tiles, channels), torch.float32, device)
+        words = _words(batch, tokens, channels)
+        states = None
+        if words:
+            states = (x.new_empty(words, dtype=torch.float32) if train
+                      else workspace.take(OP, "states", (words,), torch.float32, device))
         _fwd(device, x.data_ptr(), TYPES[x.dtype], g.data_ptr(), TYPES[g.dtype], y.data_ptr(), batch, tokens, channels,
-             *x.stride()[:2], *g.stride()[:2], pointer(cu), sequences, pointer(h0), pointer(final), pointer(scratch),
-             pointer(ends))
-    return y, final, ends
+             *x.stride()[:2], *g.stride()[:2], pointer(cu), sequences, pointer(h0), pointer(final), pointer(states))
+    return y, final, states
 
 
 def _gradients(ctx, dy, d_final):
-    x, g, h0, cu, ends = ctx.saved_tensors
+    x, g, h0, cu, states = ctx.saved_tensors
     batch, tokens, channels = x.shape
     device = x.device
     sequences = batch if cu is None else cu.numel() - 1
@@ -110,19 +109,19 @@ def _gradients(ctx, dy, d_final):
     dh0 = torch.empty_like(h0) if ctx.needs_input_grad[2] else None
     with on_device(device):
         scratch = None
-        if ends is not None:
-            scratch = workspace.take(OP, "scratch", (3, *ends.shape), torch.float32, device)
+        if states is not None:
+            scratch = workspace.take(OP, "scratch", states.shape, torch.float32, device)
         _bwd(device, dy.data_ptr(), x.data_ptr(), TYPES[x.dtype], g.data_ptr(), TYPES[g.dtype], dx.data_ptr(),
              dg.data_ptr(), batch, tokens, channels, *x.stride()[:2], *g.stride()[:2], pointer(cu), sequences,
-             pointer(h0), pointer(d_final), pointer(ends), pointer(dh0), pointer(scratch))
+             pointer(h0), pointer(d_final), pointer(states), pointer(dh0), pointer(scratch))
     return dx, dg, dh0, None, None
 
 
 class _GatedLinearRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, g, h0, cu, want_final):
-        y, final, ends = _forward(x, g, h0, cu, want_final, True)
-        ctx.save_for_backward(x, g, h0, cu, ends)
+        y, final, states = _forward(x, g, h0, cu, want_final, True)
+        ctx.save_for_backward(x, g, h0, cu, states)
         return y, final
 
     backward = staticmethod(once_differentiable(_gradients))

@@ -81,13 +81,13 @@ def test_the_library_checks_its_arguments_without_a_gpu():
 
     def fwd(x=64, x_type=0, batch=1, tokens=4, channels=8, cu=None, seqs=1):
         return lib.mek_linear_recurrence_fwd(p(x), x_type, p(64), 2, p(64), i64(batch), i64(tokens), i64(channels), i64(0),
-                                             i64(8), i64(0), i64(8), p(cu), i64(seqs), None, None, None, None, None)
+                                             i64(8), i64(0), i64(8), p(cu), i64(seqs), None, None, None, None)
 
     assert fwd(x=None) == 1 and "null" in lib.last_error()
     assert fwd(x_type=5) == 2 and "element type" in lib.last_error()
     assert fwd(tokens=0) == 1 and fwd(channels=0) == 1 and fwd(batch=0) == 1
     assert fwd(cu=64, batch=2) == 1 and "one batch row" in lib.last_error()
-    assert fwd(tokens=1 << 20) == 1 and "scratch" in lib.last_error()
+    assert fwd(tokens=1 << 20) == 1 and "no room" in lib.last_error()
     assert fwd(tokens=1 << 30, channels=1 << 23) == 1 and "tiles" in lib.last_error()
     step = lambda rows, pool, slots=None: lib.mek_linear_recurrence_step(  # noqa: E731
         p(64), 0, p(64), 0, p(64), p(slots), 0, p(64), i64(rows), i64(pool), i64(8), i64(8), i64(8), i64(8), None)
