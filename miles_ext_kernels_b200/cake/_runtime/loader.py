@@ -100,6 +100,7 @@ _COMMON_FLAGS = (
     "-Xcompiler",
     "-fPIC",
     "-shared",
+    "--threads=8",  # the sources side by side; the code does not depend on it
 )
 
 

@@ -1,0 +1,199 @@
+// The gated linear recurrence, backward (see linear_recurrence.cuh): tiles from the last to the first.  The states inside a
+// tile are recomputed from the state that entered it, which the forward's words hold; the adjoint travels through
+// words of its own.
+#include "linear_recurrence.cuh"
+
+namespace mek {
+
+struct GlrBwdArgs {
+  GlrTensor dy, x, g, dx, dg;
+  const float *h0, *d_final, *states;
+  float *words, *dh0;
+};
+
+template <typename X, typename G, bool kTma>
+__global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid_constant__ CUtensorMap dy_map,
+                                                                    const __grid_constant__ CUtensorMap x_map,
+                                                                    const __grid_constant__ CUtensorMap g_map,
+                                                                    const __grid_constant__ CUtensorMap dx_map,
+                                                                    const __grid_constant__ CUtensorMap dg_map,
+                                                                    const GlrBwdArgs p, const GlrShape s) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ GlrShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const GlrTileAt at = take_tile<true>(s, sh);
+  const int t0 = at.tile * kGlrTile + warp * kGlrTokens;
+  X* xs = reinterpret_cast<X*>(smem + warp * kGlrBox<X>);
+  X* ds = reinterpret_cast<X*>(smem + (kGlrWarps + warp) * kGlrBox<X>);
+  G* gs = reinterpret_cast<G*>(smem + 2 * kGlrWarps * kGlrBox<X> + warp * kGlrBox<G>);
+  bool arrived = true;
+  if constexpr (kTma) {
+    if (lane == 0) {
+      mbar_arrive_expect(&sh.arrived[warp], 2 * kGlrBox<X> + kGlrBox<G>);
+      box_load(gs, &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
+      box_load(ds, &dy_map, at.c0, t0, at.b, &sh.arrived[warp]);
+      box_load(xs, &x_map, at.c0, t0, at.b, &sh.arrived[warp]);
+    }
+  } else {
+    plain_load(gs, p.g, s, at, t0);
+    plain_load(ds, p.dy, s, at, t0);
+    plain_load(xs, p.x, s, at, t0);
+    __syncwarp();
+  }
+  Two h = two(0.f), c = two(0.f);
+  if (at.tile > 0) {
+    const Words v = load_words<kTma>(words_at(const_cast<float*>(p.states), s, at, at.tile - 1), s, at);
+    h = two(v.B0, v.B1);
+  }
+  const Span span = span_of(s.seq, t0);
+  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
+  const int n = min(max(s.tokens - t0, 0), kGlrTokens);
+  const uint32_t starts = span.bounds & ((1u << n) - 1), ends = (span.bounds >> 1) & ((1u << n) - 1);
+  Two a[kGlrTokens];
+  to_decays(gs, a);
+  const Words mine = fold_tokens<X, kTma>(xs, a, starts, p.h0, s, at, t0);
+  // the adjoint that leaves the warp's first token to the left: D + R c for the c that enters at its last
+  Words back;
+  {
+    Two R = two(1.f), D = two(0.f);
+    if (ends == 0) {
+#pragma unroll
+      for (int j = kGlrTokens - 1; j >= 0; --j) R = mul2(R, a[j]), D = mul2(a[j], add2(widened(token(ds, j)), D));
+    } else {
+#pragma unroll
+      for (int j = kGlrTokens - 1; j >= 0; --j) {
+        if ((ends >> j) & 1) D = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t0 + j));
+        D = mul2(a[j], add2(widened(token(ds, j)), D));
+      }
+      R = two(kGlrReset);
+    }
+    const float2 r = split(R), d = split(D);
+    back = {r.x, d.x, r.y, d.y};
+  }
+  if (!arrived) back = {kGlrReset, __int_as_float(0x7fffffff), kGlrReset, __int_as_float(0x7fffffff)};
+  const Exchange<2> ex{smem + s.exchange, s.slice};
+  __syncwarp();  // the gates are in registers: their place is free
+  ex.pair(0, warp) = make_float4(mine.A0, mine.B0, mine.A1, mine.B1);
+  ex.pair(1, warp) = make_float4(back.A0, back.B0, back.A1, back.B1);
+  __syncthreads();
+  if (s.tiles > 1) {
+    if (warp == kGlrWarps - 1) {
+#pragma unroll
+      for (int w = kGlrWarps - 2; w >= 0; --w) chain(back, ex.pair(1, w));
+      publish<kTma>(words_at(p.words, s, at, at.tile), s, at, back);
+    }
+    c = carry_in<kTma, true>(p.words, s, at, sh, ex);
+    if (warp == kGlrWarps - 1 && !back.state()) {
+      const float2 in = split(c);
+      publish<kTma>(words_at(p.words, s, at, at.tile), s, at,
+                    Words{kGlrReset, fold(back.A0, back.B0, in.x), kGlrReset, fold(back.A1, back.B1, in.y)});
+    }
+  }
+  for (int w = 0; w < warp; ++w) h = folded(ex.pair(0, w), h);
+  for (int w = kGlrWarps - 1; w > warp; --w) c = folded(ex.pair(1, w), c);
+  if (!arrived) c = two(__int_as_float(0x7fffffff));
+  __syncthreads();  // everybody has read the exchange area: dg takes the gates' place
+  Two before[kGlrTokens];  // the state before every token
+  if (span.bounds == 0 && t0 >= span.lo && t0 + kGlrTokens <= span.hi) {
+#pragma unroll
+    for (int j = 0; j < kGlrTokens; ++j) before[j] = h, h = fma2(a[j], h, widened(token(xs, j)));
+#pragma unroll
+    for (int j = kGlrTokens - 1; j >= 0; --j) {
+      const Two dh = add2(widened(token(ds, j)), c);
+      c = mul2(a[j], dh);
+      token(ds, j) = narrowed<X>(dh);
+      token(gs, j) = narrowed<G>(mul2(c, before[j]));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kGlrTokens; ++j) {
+      if ((starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t0 + j));
+      before[j] = h, h = fma2(a[j], h, widened(token(xs, j)));
+    }
+#pragma unroll
+    for (int j = kGlrTokens - 1; j >= 0; --j) {
+      const int t = t0 + j;
+      if ((ends >> j) & 1) c = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t));
+      const bool in_one = t >= span.lo && t < span.hi;
+      const Two dh = add2(widened(token(ds, j)), c);
+      c = mul2(a[j], dh);
+      token(ds, j) = narrowed<X>(in_one ? dh : two(0.f));
+      token(gs, j) = narrowed<G>(in_one ? mul2(c, before[j]) : two(0.f));
+      if (p.dh0 != nullptr && in_one && ((starts >> j) & 1))
+        store_state<kTma>(p.dh0, s, at, sequence_of(s.seq, at.b, t), c);
+    }
+  }
+  if constexpr (kTma) {
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0 && t0 < s.tokens) {
+      box_store(&dx_map, at.c0, t0, at.b, ds);
+      box_store(&dg_map, at.c0, t0, at.b, gs);
+      tma_store_commit();
+      tma_store_wait_read();
+    }
+    if (!arrived) let_copies_land();
+  } else {
+    __syncwarp();
+    plain_store(ds, p.dx, s, at, t0);
+    plain_store(gs, p.dg, s, at, t0);
+  }
+}
+
+template <typename X, typename G>
+int glr_bwd(const GlrBwdArgs& p, GlrShape s, int x_type, int g_type, bool tma, cudaStream_t stream) {
+  const char* what = "linear_recurrence_bwd";
+  const size_t smem = glr_layout<2>(s, 2 * sizeof(X) + sizeof(G), sizeof(G), 3);
+  const unsigned grid = unsigned(s.tiles) * s.channel_blocks * s.batch;
+  CUtensorMap dy_map{}, x_map{}, g_map{}, dx_map{}, dg_map{};
+  if (tma &&
+      glr_map(&dy_map, p.dy, x_type, s, what) == MEK_OK &&
+      glr_map(&x_map, p.x, x_type, s, what) == MEK_OK &&
+      glr_map(&g_map, p.g, g_type, s, what) == MEK_OK &&
+      glr_map(&dx_map, p.dx, x_type, s, what) == MEK_OK &&
+      glr_map(&dg_map, p.dg, g_type, s, what) == MEK_OK) {
+    if (int rc = want_smem(glr_bwd_kernel<X, G, true>, smem, what)) return rc;
+    glr_bwd_kernel<X, G, true><<<grid, kGlrWarps * 32, smem, stream>>>(dy_map, x_map, g_map, dx_map, dg_map, p, s);
+    return launched(what);
+  }
+  if (int rc = want_smem(glr_bwd_kernel<X, G, false>, smem, what)) return rc;
+  glr_bwd_kernel<X, G, false><<<grid, kGlrWarps * 32, smem, stream>>>(dy_map, x_map, g_map, dx_map, dg_map, p, s);
+  return launched(what);
+}
+
+}  // namespace mek
+
+extern "C" {
+
+int mek_linear_recurrence_bwd(const void* dy, const void* x, int x_type, const void* g, int g_type, void* dx, void* dg,
+                              int64_t batch, int64_t tokens, int64_t channels, int64_t x_batch_stride,
+                              int64_t x_token_stride, int64_t g_batch_stride, int64_t g_token_stride,
+                              const int32_t* cu_seqlens, int64_t num_seqs, const float* initial_state,
+                              const float* d_final_state, const float* states, float* dh0, float* scratch, void* stream) {
+  using namespace mek;
+  const char* what = "linear_recurrence_bwd";
+  if (!dy || !x || !g || !dx || !dg) return fail(MEK_ERR_INVALID, "%s: a null pointer", what);
+  if (int rc = check_glr(what, x_type, g_type, batch, tokens, channels, num_seqs, cu_seqlens)) return rc;
+  if (tokens > kGlrTile && (!scratch || !states)) return fail(MEK_ERR_INVALID, "%s: no scratch", what);
+  if ((reinterpret_cast<uintptr_t>(scratch) | reinterpret_cast<uintptr_t>(states)) % 16 != 0)
+    return fail(MEK_ERR_INVALID, "%s: states and scratch must be 16-byte aligned", what);
+  GlrShape s = glr_shape(batch, tokens, channels, num_seqs, cu_seqlens);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t dense = tokens * channels;
+  const GlrBwdArgs p{{const_cast<void*>(dy), dense, channels},
+                     {const_cast<void*>(x), x_batch_stride, x_token_stride},
+                     {const_cast<void*>(g), g_batch_stride, g_token_stride},
+                     {dx, dense, channels},
+                     {dg, dense, channels},
+                     initial_state, d_final_state, states, scratch, dh0};
+  const bool tma = glr_mappable(p.dy, x_type, s) && glr_mappable(p.x, x_type, s) && glr_mappable(p.g, g_type, s) &&
+                   glr_mappable(p.dx, x_type, s) && glr_mappable(p.dg, g_type, s) && channels % 2 == 0 &&
+                   (reinterpret_cast<uintptr_t>(initial_state) | reinterpret_cast<uintptr_t>(d_final_state) |
+                    reinterpret_cast<uintptr_t>(dh0)) % 8 == 0;
+  if (int rc = glr_clear(what, s, scratch, st)) return rc;
+  if (int rc = glr_empty(s, d_final_state, dh0, st)) return rc;
+#define MEK_GLR_BWD(X, G) glr_bwd<X, G>(p, s, x_type, g_type, tma, st)
+  MEK_GLR_TYPES(MEK_GLR_BWD);
+}
+
+}  // extern "C"

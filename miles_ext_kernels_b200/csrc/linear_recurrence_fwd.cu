@@ -1,0 +1,152 @@
+// The gated linear recurrence, forward (see linear_recurrence.cuh).
+#include "linear_recurrence.cuh"
+
+namespace mek {
+
+struct GlrFwdArgs {
+  GlrTensor x, g, y;
+  const float* h0;
+  float *words, *final_state;
+};
+
+template <typename X, typename G, bool kTma>
+__global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid_constant__ CUtensorMap x_map,
+                                                                    const __grid_constant__ CUtensorMap g_map,
+                                                                    const __grid_constant__ CUtensorMap y_map,
+                                                                    const GlrFwdArgs p, const GlrShape s) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ GlrShared sh;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const GlrTileAt at = take_tile<false>(s, sh);
+  const int t0 = at.tile * kGlrTile + warp * kGlrTokens;
+  X* xs = reinterpret_cast<X*>(smem + warp * kGlrBox<X>);
+  G* gs = reinterpret_cast<G*>(smem + kGlrWarps * kGlrBox<X> + warp * kGlrBox<G>);
+  bool arrived = true;
+  if constexpr (kTma) {
+    if (lane == 0) {
+      mbar_arrive_expect(&sh.arrived[warp], kGlrBox<X> + kGlrBox<G>);
+      box_load(gs, &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
+      box_load(xs, &x_map, at.c0, t0, at.b, &sh.arrived[warp]);
+    }
+  } else {
+    plain_load(gs, p.g, s, at, t0);
+    plain_load(xs, p.x, s, at, t0);
+    __syncwarp();
+  }
+  const Span span = span_of(s.seq, t0);
+  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
+  const int n = min(max(s.tokens - t0, 0), kGlrTokens);
+  const uint32_t starts = span.bounds & ((1u << n) - 1);
+  Two a[kGlrTokens];
+  to_decays(gs, a);
+  Words tile = fold_tokens<X, kTma>(xs, a, starts, p.h0, s, at, t0);
+  if (!arrived) tile = {kGlrReset, __int_as_float(0x7fffffff), kGlrReset, __int_as_float(0x7fffffff)};
+  Two h = two(0.f);
+  if (s.tiles > 1) {
+    const Exchange<1> ex{smem + s.exchange, s.slice};
+    __syncwarp();  // the gates are in registers: their place is free
+    ex.pair(0, warp) = make_float4(tile.A0, tile.B0, tile.A1, tile.B1);
+    __syncthreads();
+    if (warp == 0) {
+#pragma unroll
+      for (int w = 1; w < kGlrWarps; ++w) chain(tile, ex.pair(0, w));
+      publish<kTma>(words_at(p.words, s, at, at.tile), s, at, tile);
+    }
+    h = carry_in<kTma, false>(p.words, s, at, sh, ex);
+    if (warp == 0 && !tile.state()) {
+      const float2 in = split(h);
+      publish<kTma>(words_at(p.words, s, at, at.tile), s, at,
+                    Words{kGlrReset, fold(tile.A0, tile.B0, in.x), kGlrReset, fold(tile.A1, tile.B1, in.y)});
+    }
+    for (int w = 0; w < warp; ++w) h = folded(ex.pair(0, w), h);
+  } else {
+    const Exchange<1> ex{smem + s.exchange, s.slice};
+    __syncwarp();
+    ex.pair(0, warp) = make_float4(tile.A0, tile.B0, tile.A1, tile.B1);
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) h = folded(ex.pair(0, w), h);
+  }
+  if (!arrived) h = two(__int_as_float(0x7fffffff));
+  if (span.bounds == 0 && t0 >= span.lo && t0 + kGlrTokens <= span.hi) {  // all of one sequence, which goes on
+#pragma unroll
+    for (int j = 0; j < kGlrTokens; ++j) {
+      h = fma2(a[j], h, widened(token(xs, j)));
+      token(xs, j) = narrowed<X>(h);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kGlrTokens; ++j) {
+      const int t = t0 + j;
+      if ((starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t));
+      h = fma2(a[j], h, widened(token(xs, j)));
+      const bool in_one = t >= span.lo && t < span.hi;
+      token(xs, j) = narrowed<X>(in_one ? h : two(0.f));
+      if (p.final_state != nullptr && in_one && span.ends(j))
+        store_state<kTma>(p.final_state, s, at, sequence_of(s.seq, at.b, t), h);
+    }
+  }
+  if constexpr (kTma) {
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0 && t0 < s.tokens) {
+      box_store(&y_map, at.c0, t0, at.b, xs);
+      tma_store_commit();
+      tma_store_wait_read();
+    }
+    if (!arrived) let_copies_land();
+  } else {
+    __syncwarp();
+    plain_store(xs, p.y, s, at, t0);
+  }
+}
+
+template <typename X, typename G>
+int glr_fwd(const GlrFwdArgs& p, GlrShape s, int x_type, int g_type, bool tma, cudaStream_t stream) {
+  const char* what = "linear_recurrence_fwd";
+  const size_t smem = glr_layout<1>(s, sizeof(X) + sizeof(G), sizeof(G), 4);
+  const unsigned grid = unsigned(s.tiles) * s.channel_blocks * s.batch;
+  CUtensorMap x_map{}, g_map{}, y_map{};
+  if (tma &&
+      glr_map(&x_map, p.x, x_type, s, what) == MEK_OK &&
+      glr_map(&g_map, p.g, g_type, s, what) == MEK_OK &&
+      glr_map(&y_map, p.y, x_type, s, what) == MEK_OK) {
+    if (int rc = want_smem(glr_fwd_kernel<X, G, true>, smem, what)) return rc;
+    glr_fwd_kernel<X, G, true><<<grid, kGlrWarps * 32, smem, stream>>>(x_map, g_map, y_map, p, s);
+    return launched(what);
+  }
+  if (int rc = want_smem(glr_fwd_kernel<X, G, false>, smem, what)) return rc;
+  glr_fwd_kernel<X, G, false><<<grid, kGlrWarps * 32, smem, stream>>>(x_map, g_map, y_map, p, s);
+  return launched(what);
+}
+
+}  // namespace mek
+
+extern "C" {
+
+int mek_linear_recurrence_tile(void) { return mek::kGlrTile; }
+
+int mek_linear_recurrence_fwd(const void* x, int x_type, const void* g, int g_type, void* y, int64_t batch,
+                              int64_t tokens, int64_t channels, int64_t x_batch_stride, int64_t x_token_stride,
+                              int64_t g_batch_stride, int64_t g_token_stride, const int32_t* cu_seqlens, int64_t num_seqs,
+                              const float* initial_state, float* final_state, float* states, void* stream) {
+  using namespace mek;
+  const char* what = "linear_recurrence_fwd";
+  if (!x || !g || !y) return fail(MEK_ERR_INVALID, "%s: a null pointer", what);
+  if (int rc = check_glr(what, x_type, g_type, batch, tokens, channels, num_seqs, cu_seqlens)) return rc;
+  if (tokens > kGlrTile && !states) return fail(MEK_ERR_INVALID, "%s: no room for the tiles' states", what);
+  if (reinterpret_cast<uintptr_t>(states) % 16 != 0) return fail(MEK_ERR_INVALID, "%s: states must be 16-byte aligned", what);
+  GlrShape s = glr_shape(batch, tokens, channels, num_seqs, cu_seqlens);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const GlrFwdArgs p{{const_cast<void*>(x), x_batch_stride, x_token_stride},
+                     {const_cast<void*>(g), g_batch_stride, g_token_stride},
+                     {y, tokens * channels, channels},
+                     initial_state, states, final_state};
+  const bool tma = glr_mappable(p.x, x_type, s) && glr_mappable(p.g, g_type, s) && glr_mappable(p.y, x_type, s) &&
+                   channels % 2 == 0 && (reinterpret_cast<uintptr_t>(initial_state) | reinterpret_cast<uintptr_t>(final_state)) % 8 == 0;
+  if (int rc = glr_clear(what, s, states, st)) return rc;
+  if (int rc = glr_empty(s, initial_state, final_state, st)) return rc;
+#define MEK_GLR_FWD(X, G) glr_fwd<X, G>(p, s, x_type, g_type, tma, st)
+  MEK_GLR_TYPES(MEK_GLR_FWD);
+}
+
+}  // extern "C"
