@@ -68,33 +68,39 @@ __device__ __forceinline__ Two add2(Two a, Two b) {
   return d;
 }
 
-// exp(g) from its Taylor series about zero after a reduction by multiples of log 2: the last operation rounds 1 + p once,
-// so a decay next to one carries no bias.  (CUDA's expf is off by up to an ulp to one side there, and a thousand tokens'
-// memory adds that up: relative error of a state 7e-6 with expf, 4e-7 with this.)  The remainder of degree 7 at
-// |r| <= log(2) / 2 is below 6e-9.  For |g| <= 87; the nearest integer n sits in the low bits of the shifted product, so
-// 2^n is added to the exponent with one multiply-add.
-constexpr float kDecayRange = 87.f;
-__device__ __forceinline__ Two decays_in_range(Two g) {
-  const Two shifted = fma2(g, two(1.44269504f), two(12582912.f));
-  const Two n = add2(shifted, two(-12582912.f));
-  Two r = fma2(n, two(-0.693359375f), g);  // log 2 in two parts, the first exact
-  r = fma2(n, two(2.12194440e-4f), r);
-  Two q = fma2(r, two(1.f / 5040.f), two(1.f / 720.f));
-  q = fma2(q, r, two(1.f / 120.f));
-  q = fma2(q, r, two(1.f / 24.f));
-  q = fma2(q, r, two(1.f / 6.f));
+__device__ __forceinline__ Two sub2(Two a, Two b) {
+  Two d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+__device__ __forceinline__ float clamped(float g) {  // NaN stays
+  float v;
+  asm("max.NaN.f32 %0, %1, 0fC2B00000;" : "=f"(v) : "f"(g));   // -88
+  asm("min.NaN.f32 %0, %1, 0f42B1999A;" : "=f"(v) : "f"(v));   // 88.8
+  return v;
+}
+
+// exp(g) = 2^n (1 + r + r^2 q(r)), r = g - n log 2: 1 + p is rounded once, so a decay next to one carries no bias.  (CUDA's
+// expf is off by up to an ulp to one side there, and a thousand tokens' memory adds that up: relative error of a state
+// 7e-6 with expf, 4e-7 with this.)  q of degree 4 is the minimax fit of (e^r - 1 - r) / r^2 over |r| <= log(2) / 2 in
+// the error of the whole, found by reweighted least squares: off by at most 5.3e-9, by 2e-10 for |r| < 0.05.  The
+// rounding of log 2 puts |n| 2e-9 into the relative error: at n = 1 the memory is a token long already.
+// n sits in the low bits of the shifted product, from where one multiply-add makes 2^n: for the clamped range between
+// n = -127, whose bits are zero (a gate at or below -88, minus infinity too, closes exactly), and n = 128, infinity.
+__device__ __forceinline__ Two decays(Two gates) {
+  const float2 v = split(gates);
+  const Two g = two(clamped(v.x), clamped(v.y)), shift = two(12582912.f);
+  const Two shifted = fma2(g, two(1.44269504f), shift);
+  const Two n = sub2(shifted, shift), r = fma2(n, two(-0.693147181f), g);
+  Two q = fma2(r, two(0.00139505253f), two(0.00836891122f));
+  q = fma2(q, r, two(0.0416662060f));
+  q = fma2(q, r, two(0.166665182f));
   q = fma2(q, r, two(0.5f));
-  const float2 e = split(add2(fma2(mul2(r, r), q, r), two(1.f))), k = split(shifted);
-  return two(__int_as_float(__float_as_int(k.x) * (1 << 23) + __float_as_int(e.x)),
-             __int_as_float(__float_as_int(k.y) * (1 << 23) + __float_as_int(e.y)));
-}
-// Any g: below -87 the result is zero, above log(FLT_MAX) infinity; NaN stays NaN.
-__device__ __forceinline__ float decay_fixed(float g, float e) {
-  return g < -kDecayRange ? 0.f : g <= 88.7228f ? e : g + __int_as_float(0x7f800000);
-}
-__device__ __forceinline__ Two decays(Two g) {
-  const float2 v = split(g), e = split(decays_in_range(g));
-  return two(decay_fixed(v.x, e.x), decay_fixed(v.y, e.y));
+  const Two e = add2(fma2(mul2(r, r), q, r), two(1.f));
+  const float2 m = split(shifted);
+  return mul2(e, two(__int_as_float(__float_as_int(m.x) * (1 << 23) + 0x3f800000),
+                     __int_as_float(__float_as_int(m.y) * (1 << 23) + 0x3f800000)));
 }
 
 __device__ __forceinline__ float fold(float A, float B, float h) { return A < 0.f ? B : fmaf(A, h, B); }
@@ -175,9 +181,7 @@ struct GlrTensor {
 struct GlrShape {
   Sequences seq;
   int batch, tokens, channels, tiles, channel_blocks;
-  int window;        // words a warp looks back over at once
-  int slice;         // bytes of a warp's part of the exchange area
-  int exchange;      // where that area starts in dynamic shared memory
+  int window;        // words a warp looks back over at once; 0: one warp looks at the nearest four
   int* counter;      // the last tile taken (-1 before the launch); NULL where there is one tile a chain
 };
 struct GlrTileAt {
@@ -191,24 +195,30 @@ __device__ __forceinline__ GlrTileAt tile_at(const GlrShape& s, int index) {
   return {chain / s.channel_blocks, kReverse ? s.tiles - 1 - step : step, (chain % s.channel_blocks) * kGlrChannels};
 }
 
+// What the warps of a block exchange.
+template <int kDirections>
 struct GlrShared {
-  uint64_t arrived[kGlrWarps];  // a warp's boxes
-  int2 marks[kGlrWarps];        // nearest word not set, nearest state, among the words a warp looked at
-  int ticket, late;
+  float4 pair[kDirections][kGlrWarps][32];  // the warps' (A0, B0, A1, B1)
+  Two carried[32];                          // the state that enters the tile
+  uint64_t arrived[kGlrWarps];              // a warp's boxes
+  int2 marks[kGlrWarps];                    // nearest word not set, nearest state, among the words a warp looked at
+  GlrTileAt at;
+  int late;
 };
 
 // The block's tile -- the next in order, or its own index where tiles do not wait for one another -- and the barriers.
-template <bool kReverse>
-__device__ __forceinline__ GlrTileAt take_tile(const GlrShape& s, GlrShared& sh) {
-  if (threadIdx.x == 0) {
-    sh.ticket = s.counter ? atomicAdd(s.counter, 1) + 1 : int(blockIdx.x);
-    sh.late = 0;
-#pragma unroll
-    for (int w = 0; w < kGlrWarps; ++w) mbar_init(&sh.arrived[w], 1);
+template <bool kReverse, int kDirections>
+__device__ __forceinline__ GlrTileAt take_tile(const GlrShape& s, GlrShared<kDirections>& sh) {
+  if (threadIdx.x < 32) {
+    if (threadIdx.x < kGlrWarps) mbar_init(&sh.arrived[threadIdx.x], 1);
     fence_mbar_init();
+    if (threadIdx.x == 0) {
+      sh.at = tile_at<kReverse>(s, s.counter ? atomicAdd(s.counter, 1) + 1 : int(blockIdx.x));
+      sh.late = 0;
+    }
   }
   __syncthreads();
-  return tile_at<kReverse>(s, sh.ticket);
+  return sh.at;
 }
 
 // ---- tokens between global memory and a warp's shared tile [16][64] -------------------------------------------------
@@ -328,28 +338,46 @@ __device__ __forceinline__ void publish(float* row, const GlrShape& s, const Glr
   }
 }
 
-// The exchange area: per warp kDirections pairs (A0, B0, A1, B1) of 32 lanes, then the words the warp looked at.  It lies
-// in the shared tiles of the gates where it fits: they are in registers by then.
-template <int kDirections>
-struct Exchange {
-  uint8_t* base;
-  int slice;
-  __device__ __forceinline__ float4& pair(int direction, int warp) const {
-    return reinterpret_cast<float4*>(base + warp * slice)[direction * 32 + (threadIdx.x & 31)];
+// Looking back with one warp: the nearest state among the four tiles before this one.
+constexpr int kGlrNear = 4;
+template <bool kPair, bool kReverse>
+__device__ __forceinline__ Two look_back(float* words, const GlrShape& s, const GlrTileAt& at, int before) {
+  const uint64_t began = global_timer_ns();
+  const float* row = words_at(words, s, at, at.tile);
+  const int64_t step = int64_t(kReverse ? 2 : -2) * s.channels;
+  for (;;) {
+    Words v[kGlrNear];
+#pragma unroll
+    for (int k = 0; k < kGlrNear; ++k) {
+      v[k] = {kGlrReset, 0.f, kGlrReset, 0.f};  // before the first tile: a state of zero
+      if (k < before) v[k] = load_words<kPair>(row + (k + 1) * step, s, at);
+    }
+    bool ready = true;
+    float h[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kGlrNear; ++k) {
+      ready = ready && __all_sync(0xffffffffu, v[k].set());
+      if (!ready) break;
+      if (__all_sync(0xffffffffu, v[k].state())) {
+#pragma unroll
+        for (int i = kGlrNear - 1; i >= 0; --i)
+          if (i <= k) h[0] = fold(v[i].A0, v[i].B0, h[0]), h[1] = fold(v[i].A1, v[i].B1, h[1]);
+        return two(h[0], h[1]);
+      }
+    }
+    if (global_timer_ns() - began > kWaitLimitNs) return two(__int_as_float(0x7fffffff));
   }
-  __device__ __forceinline__ float4& look(int warp, int k) const {
-    return reinterpret_cast<float4*>(base + warp * slice)[(kDirections + k) * 32 + (threadIdx.x & 31)];
-  }
-};
+}
 
-// The state that enters the tile (from the left; reversed: the adjoint from the right), in every warp.  Called by the
-// whole block after one warp has published the tile's own pair.
+// Looking back with the whole block, for chains whose tiles in flight lie far behind one another: warp w looks at the words
+// behind those of warp w - 1 until there is a state with no unset word in front of it; `owner` then folds forward from
+// it, reading the words again (a word that has become a state since gives the same bits).  Only the owner's result counts.
 template <bool kPair, bool kReverse, int kDirections>
-__device__ __forceinline__ Two carry_in(float* words, const GlrShape& s, const GlrTileAt& at, GlrShared& sh,
-                                        const Exchange<kDirections>& ex) {
-  const int before = kReverse ? s.tiles - 1 - at.tile : at.tile;  // tiles that come before this one
-  if (before == 0) return two(0.f);
+__device__ __forceinline__ Two look_back_together(float* words, const GlrShape& s, const GlrTileAt& at,
+                                                  GlrShared<kDirections>& sh, int before, int owner) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float* row = words_at(words, s, at, at.tile);
+  const int64_t step = int64_t(kReverse ? 2 : -2) * s.channels;
   constexpr int kFar = 0x7fffffff;
   uint64_t began = 0;
   int from;
@@ -358,9 +386,7 @@ __device__ __forceinline__ Two carry_in(float* words, const GlrShape& s, const G
     for (int k = 0; k < s.window; ++k) {
       const int back = warp * s.window + k;
       Words v{kGlrReset, 0.f, kGlrReset, 0.f};  // before the first tile: a state of zero
-      if (back < before)
-        v = load_words<kPair>(words_at(words, s, at, kReverse ? at.tile + 1 + back : at.tile - 1 - back), s, at);
-      ex.look(warp, k) = make_float4(v.A0, v.B0, v.A1, v.B1);
+      if (back < before) v = load_words<kPair>(row + (back + 1) * step, s, at);
       if (!__all_sync(0xffffffffu, v.set())) unset = min(unset, back);
       else if (__all_sync(0xffffffffu, v.state())) state = min(state, back);
     }
@@ -376,15 +402,49 @@ __device__ __forceinline__ Two carry_in(float* words, const GlrShape& s, const G
     const bool late = sh.late != 0;
     if (from < unset) break;
     if (late) return two(__int_as_float(0x7fffffff));
-    __syncthreads();  // before the words are looked at again
+    __syncthreads();  // before the marks are set again
   }
   float h[2] = {0.f, 0.f};
-  for (int w = from / s.window, k = from % s.window; w >= 0; --w, k = s.window - 1)
-    for (; k >= 0; --k) {
-      const float4 v = ex.look(w, k);
-      h[0] = fold(v.x, v.y, h[0]), h[1] = fold(v.z, v.w, h[1]);
+  if (warp == owner) {
+    for (; from >= 0; from -= kGlrNear) {
+      Words v[kGlrNear];
+#pragma unroll
+      for (int k = 0; k < kGlrNear; ++k) {
+        v[k] = {kGlrReset, h[0], kGlrReset, h[1]};
+        const int back = from - k;
+        if (back >= 0 && back < before) v[k] = load_words<kPair>(row + (back + 1) * step, s, at);
+        else if (back >= 0) v[k] = {kGlrReset, 0.f, kGlrReset, 0.f};
+      }
+#pragma unroll
+      for (int k = 0; k < kGlrNear; ++k)
+        if (from - k >= 0) h[0] = fold(v[k].A0, v[k].B0, h[0]), h[1] = fold(v[k].A1, v[k].B1, h[1]);
     }
+  }
   return two(h[0], h[1]);
+}
+
+// The state that enters the tile (from the left; reversed: the adjoint from the right), in every warp.  Called by the
+// whole block after its warp `owner` has published the tile's own pair `tile`; that warp then publishes the state.
+template <bool kPair, bool kReverse, int kDirections>
+__device__ __forceinline__ Two carry_in(float* words, const GlrShape& s, const GlrTileAt& at, GlrShared<kDirections>& sh,
+                                        int owner, const Words& tile) {
+  const int before = kReverse ? s.tiles - 1 - at.tile : at.tile;  // tiles that come before this one
+  const bool mine = int(threadIdx.x >> 5) == owner;
+  Two h = two(0.f);
+  if (before > 0) {
+    if (s.window > 0) h = look_back_together<kPair, kReverse>(words, s, at, sh, before, owner);
+    else if (mine) h = look_back<kPair, kReverse>(words, s, at, before);
+  }
+  if (mine) {
+    if (!tile.state()) {  // else it was one already
+      const float2 in = split(h);
+      publish<kPair>(words_at(words, s, at, at.tile), s, at,
+                     Words{kGlrReset, fold(tile.A0, tile.B0, in.x), kGlrReset, fold(tile.A1, tile.B1, in.y)});
+    }
+    sh.carried[threadIdx.x & 31] = h;
+  }
+  __syncthreads();
+  return sh.carried[threadIdx.x & 31];
 }
 __device__ __forceinline__ Two folded(const float4& v, Two h) {
   const float2 f = split(h);
@@ -395,42 +455,73 @@ __device__ __forceinline__ void chain(Words& v, const float4& w) {
   chain(v.A1, v.B1, w.z, w.w);
 }
 
-// The decays of the warp's tokens from their gates.
+// A warp's gates and, once they are exponentiated, its decays [16][64] in FP32, in one place.  16-bit gates arrive in the
+// upper half (token j's at byte 2,048 + 128 j): from token 8 on, token j's decays (byte 256 j) overwrite gates of tokens
+// 2 j - 16 and 2 j - 15, none later than j.  Gradients of 16-bit gates go to the upper half again, token j's over the
+// decays of token 8 + j / 2, none earlier than j on the way back.  A warp's lanes are brought together before each such
+// write, so that all have read what it overwrites; FP32 gates and their gradients lie in the lane's own decay.
+constexpr uint32_t kGlrDecays = kGlrTokens * kGlrChannels * sizeof(float);
 template <typename G>
-__device__ __forceinline__ void to_decays(G* gates, Two (&a)[kGlrTokens]) {
-  bool plain = true;
-#pragma unroll
-  for (int j = 0; j < kGlrTokens; ++j) {
-    const Two g = widened(token(gates, j));
-    const float2 v = split(g);
-    plain &= fabsf(v.x) <= kDecayRange && fabsf(v.y) <= kDecayRange;  // false for NaN
-    a[j] = decays_in_range(g);
-  }
-  if (!__all_sync(0xffffffffu, plain)) {
-#pragma unroll
-    for (int j = 0; j < kGlrTokens; ++j) a[j] = decays(widened(token(gates, j)));
-  }
+__device__ __forceinline__ G* gates_of(float* decays) {
+  return reinterpret_cast<G*>(reinterpret_cast<uint8_t*>(decays) + kGlrDecays - kGlrBox<G>);
+}
+__device__ __forceinline__ Two decay_at(const float* decays, int j) {
+  return *reinterpret_cast<const Two*>(decays + j * kGlrChannels + 2 * (threadIdx.x & 31));
 }
 
-// (A, B) of the warp's tokens; starts: its tokens that begin a sequence.
-template <typename X, bool kPair>
-__device__ __forceinline__ Words fold_tokens(X* xs, const Two (&a)[kGlrTokens], uint32_t starts, const float* __restrict__ h0,
-                                             const GlrShape& s, const GlrTileAt& at, int t0) {
-  Two A = two(1.f), B = two(0.f);
-  if (starts == 0) {
-#pragma unroll
-    for (int j = 0; j < kGlrTokens; ++j) A = mul2(A, a[j]), B = fma2(a[j], B, widened(token(xs, j)));
-  } else {
-#pragma unroll
-    for (int j = 0; j < kGlrTokens; ++j) {
-      if ((starts >> j) & 1) B = load_state<kPair>(h0, s, at, sequence_of(s.seq, at.b, t0 + j));
-      B = fma2(a[j], B, widened(token(xs, j)));
-    }
-    A = two(kGlrReset);
-  }
-  const float2 p = split(A), q = split(B);
-  return {p.x, q.x, p.y, q.y};
+template <typename G>
+__device__ __forceinline__ void put_decay(float* decays, int j, Two a) {
+  if (sizeof(G) < sizeof(float) && j >= kGlrTokens / 2) __syncwarp();
+  *reinterpret_cast<Two*>(decays + j * kGlrChannels + 2 * (threadIdx.x & 31)) = a;
 }
+template <typename G>
+__device__ __forceinline__ void put_gradient(float* decays, int j, Two dg) {
+  if (sizeof(G) < sizeof(float)) __syncwarp();
+  token(gates_of<G>(decays), j) = narrowed<G>(dg);
+}
+
+// One walk over the warp's tokens: gates to decays, and the fold of the run to (A, B); with gradients ds (kBack) also to
+// (A, D), D the adjoint that leaves the first token to the left when nothing enters at the last.
+template <typename X, typename G, bool kBack>
+__device__ __forceinline__ void walk_tokens(float* decay, X* xs, X* ds, Two& A, Two& B, Two& D) {
+  G* gates = gates_of<G>(decay);
+  A = two(1.f), B = D = two(0.f);
+#pragma unroll
+  for (int j = 0; j < kGlrTokens; ++j) {
+    const Two a = decays(widened(token(gates, j)));
+    put_decay<G>(decay, j, a);
+    A = mul2(A, a);
+    B = fma2(a, B, widened(token(xs, j)));
+    if constexpr (kBack) D = fma2(A, widened(token(ds, j)), D);
+  }
+}
+// The same folds where sequences start or end among the tokens; a fold that meets a boundary does not depend on what
+// comes before (A < 0).
+template <typename X, bool kPair>
+__device__ __forceinline__ void fold_from_starts(const float* decay, X* xs, uint32_t starts, const float* __restrict__ h0,
+                                                 const GlrShape& s, const GlrTileAt& at, int t0, Two& A, Two& B) {
+  B = two(0.f), A = two(kGlrReset);
+#pragma unroll 4
+  for (int j = 0; j < kGlrTokens; ++j) {
+    if ((starts >> j) & 1) B = load_state<kPair>(h0, s, at, sequence_of(s.seq, at.b, t0 + j));
+    B = fma2(decay_at(decay, j), B, widened(token(xs, j)));
+  }
+}
+template <typename X, bool kPair>
+__device__ __forceinline__ void fold_from_ends(const float* decay, X* ds, uint32_t ends, const float* __restrict__ d_final,
+                                               const GlrShape& s, const GlrTileAt& at, int t0, Two& A, Two& D) {
+  D = two(0.f), A = two(kGlrReset);
+#pragma unroll 4
+  for (int j = kGlrTokens - 1; j >= 0; --j) {
+    if ((ends >> j) & 1) D = load_state<kPair>(d_final, s, at, sequence_of(s.seq, at.b, t0 + j));
+    D = mul2(decay_at(decay, j), add2(widened(token(ds, j)), D));
+  }
+}
+__device__ __forceinline__ float4 packed(Two A, Two B) {
+  const float2 a = split(A), b = split(B);
+  return make_float4(a.x, b.x, a.y, b.y);
+}
+__device__ __forceinline__ Words words_of(const float4& v) { return {v.x, v.y, v.z, v.w}; }
 
 // After a wait that ran out: copies that are still in flight may write to this block's shared memory.
 __device__ __forceinline__ void let_copies_land() {
@@ -456,24 +547,16 @@ inline int size_of(int type) { return type == kTypeFp32 ? 4 : 2; }
 
 inline GlrShape glr_shape(int64_t batch, int64_t tokens, int64_t channels, int64_t seqs, const int32_t* cu) {
   return {{cu, int(cu ? seqs : batch), int(tokens)}, int(batch), int(tokens), int(channels),
-          int((tokens + kGlrTile - 1) / kGlrTile), int((channels + kGlrChannels - 1) / kGlrChannels), 1, 0, 0, nullptr};
+          int((tokens + kGlrTile - 1) / kGlrTile), int((channels + kGlrChannels - 1) / kGlrChannels), 0, nullptr};
 }
 
-// Shared memory of a launch: the tiles of `tensors` bytes a token and channel (the gates' last), then the exchange area
-// unless it fits into the gates' tiles.  The window: words a warp looks back over, eight warps together.  With few
-// chains (channel blocks x batch rows) the tiles in flight lie one behind the other, so the nearest state may be as
-// many tiles back as there are blocks on the GPU per chain; with many chains it is near, and a wide window would only
-// read more.
-template <int kDirections>
-size_t glr_layout(GlrShape& s, int tensors, int gate_size, int blocks_per_sm) {
+// The window: words a warp looks back over, eight warps together.  With few chains (channel blocks x batch rows) the tiles
+// in flight lie one behind the other, so the nearest state may be as many tiles back as there are blocks on the GPU per
+// chain; where it is at most four tiles back, one warp looks (window 0) and the others wait, which saves their
+// instructions.
+inline void glr_window(GlrShape& s, int blocks_per_sm) {
   const int64_t chains = int64_t(s.batch) * s.channel_blocks, depth = (blocks_per_sm * 148 + chains - 1) / chains;
-  s.window = int(depth >= 6 * kGlrWarps ? 6 : depth <= kGlrWarps ? 1 : (depth + kGlrWarps - 1) / kGlrWarps);
-  const int need = 32 * int(sizeof(float4)) * (kDirections + s.window);
-  const int tiles = kGlrTile * kGlrChannels * tensors, gates = kGlrTokens * kGlrChannels * gate_size;
-  const bool inside = need <= gates;
-  s.slice = inside ? gates : need;
-  s.exchange = inside ? tiles - kGlrTile * kGlrChannels * gate_size : tiles;
-  return inside ? tiles : tiles + need * kGlrWarps;
+  s.window = int(depth >= 6 * kGlrWarps ? 6 : depth <= kGlrNear ? 0 : (depth + kGlrWarps - 1) / kGlrWarps);
 }
 
 // Words unset and the counter behind them at -1: one asynchronous fill with ones (nothing where a chain is one tile).

@@ -19,13 +19,14 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
                                                                     const __grid_constant__ CUtensorMap dg_map,
                                                                     const GlrBwdArgs p, const GlrShape s) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ GlrShared sh;
+  __shared__ GlrShared<2> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const GlrTileAt at = take_tile<true>(s, sh);
   const int t0 = at.tile * kGlrTile + warp * kGlrTokens;
-  X* xs = reinterpret_cast<X*>(smem + warp * kGlrBox<X>);
-  X* ds = reinterpret_cast<X*>(smem + (kGlrWarps + warp) * kGlrBox<X>);
-  G* gs = reinterpret_cast<G*>(smem + 2 * kGlrWarps * kGlrBox<X> + warp * kGlrBox<G>);
+  float* decay = reinterpret_cast<float*>(smem + warp * kGlrDecays);
+  X* xs = reinterpret_cast<X*>(smem + kGlrWarps * kGlrDecays + warp * kGlrBox<X>);
+  X* ds = reinterpret_cast<X*>(smem + kGlrWarps * (kGlrDecays + kGlrBox<X>) + warp * kGlrBox<X>);
+  G* gs = gates_of<G>(decay);
   bool arrived = true;
   if constexpr (kTma) {
     if (lane == 0) {
@@ -46,69 +47,49 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
     h = two(v.B0, v.B1);
   }
   const Span span = span_of(s.seq, t0);
-  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
   const int n = min(max(s.tokens - t0, 0), kGlrTokens);
   const uint32_t starts = span.bounds & ((1u << n) - 1), ends = (span.bounds >> 1) & ((1u << n) - 1);
-  Two a[kGlrTokens];
-  to_decays(gs, a);
-  const Words mine = fold_tokens<X, kTma>(xs, a, starts, p.h0, s, at, t0);
-  // the adjoint that leaves the warp's first token to the left: D + R c for the c that enters at its last
-  Words back;
+  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
   {
-    Two R = two(1.f), D = two(0.f);
-    if (ends == 0) {
-#pragma unroll
-      for (int j = kGlrTokens - 1; j >= 0; --j) R = mul2(R, a[j]), D = mul2(a[j], add2(widened(token(ds, j)), D));
-    } else {
-#pragma unroll
-      for (int j = kGlrTokens - 1; j >= 0; --j) {
-        if ((ends >> j) & 1) D = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t0 + j));
-        D = mul2(a[j], add2(widened(token(ds, j)), D));
-      }
-      R = two(kGlrReset);
-    }
-    const float2 r = split(R), d = split(D);
-    back = {r.x, d.x, r.y, d.y};
+    Two A, B, D;
+    walk_tokens<X, G, true>(decay, xs, ds, A, B, D);
+    Two R = A;
+    if (starts) fold_from_starts<X, kTma>(decay, xs, starts, p.h0, s, at, t0, A, B);
+    if (ends) fold_from_ends<X, kTma>(decay, ds, ends, p.d_final, s, at, t0, R, D);
+    if (!arrived) R = two(kGlrReset), D = two(__int_as_float(0x7fffffff));
+    sh.pair[0][warp][lane] = packed(A, B);
+    sh.pair[1][warp][lane] = packed(R, D);
   }
-  if (!arrived) back = {kGlrReset, __int_as_float(0x7fffffff), kGlrReset, __int_as_float(0x7fffffff)};
-  const Exchange<2> ex{smem + s.exchange, s.slice};
-  __syncwarp();  // the gates are in registers: their place is free
-  ex.pair(0, warp) = make_float4(mine.A0, mine.B0, mine.A1, mine.B1);
-  ex.pair(1, warp) = make_float4(back.A0, back.B0, back.A1, back.B1);
   __syncthreads();
   if (s.tiles > 1) {
+    Words tile = words_of(sh.pair[1][kGlrWarps - 1][lane]);
     if (warp == kGlrWarps - 1) {
 #pragma unroll
-      for (int w = kGlrWarps - 2; w >= 0; --w) chain(back, ex.pair(1, w));
-      publish<kTma>(words_at(p.words, s, at, at.tile), s, at, back);
+      for (int w = kGlrWarps - 2; w >= 0; --w) chain(tile, sh.pair[1][w][lane]);
+      publish<kTma>(words_at(p.words, s, at, at.tile), s, at, tile);
     }
-    c = carry_in<kTma, true>(p.words, s, at, sh, ex);
-    if (warp == kGlrWarps - 1 && !back.state()) {
-      const float2 in = split(c);
-      publish<kTma>(words_at(p.words, s, at, at.tile), s, at,
-                    Words{kGlrReset, fold(back.A0, back.B0, in.x), kGlrReset, fold(back.A1, back.B1, in.y)});
-    }
+    c = carry_in<kTma, true>(p.words, s, at, sh, kGlrWarps - 1, tile);
   }
-  for (int w = 0; w < warp; ++w) h = folded(ex.pair(0, w), h);
-  for (int w = kGlrWarps - 1; w > warp; --w) c = folded(ex.pair(1, w), c);
+  for (int w = 0; w < warp; ++w) h = folded(sh.pair[0][w][lane], h);
+  for (int w = kGlrWarps - 1; w > warp; --w) c = folded(sh.pair[1][w][lane], c);
   if (!arrived) c = two(__int_as_float(0x7fffffff));
-  __syncthreads();  // everybody has read the exchange area: dg takes the gates' place
-  Two before[kGlrTokens];  // the state before every token
+  // forward once more for the state before every token, then back with the adjoint; dx takes dy's place, dg the gates'
+  Two before[kGlrTokens];
   if (span.bounds == 0 && t0 >= span.lo && t0 + kGlrTokens <= span.hi) {
 #pragma unroll
-    for (int j = 0; j < kGlrTokens; ++j) before[j] = h, h = fma2(a[j], h, widened(token(xs, j)));
+    for (int j = 0; j < kGlrTokens; ++j) before[j] = h, h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
 #pragma unroll
     for (int j = kGlrTokens - 1; j >= 0; --j) {
       const Two dh = add2(widened(token(ds, j)), c);
-      c = mul2(a[j], dh);
+      c = mul2(decay_at(decay, j), dh);
       token(ds, j) = narrowed<X>(dh);
-      token(gs, j) = narrowed<G>(mul2(c, before[j]));
+      put_gradient<G>(decay, j, mul2(c, before[j]));
     }
   } else {
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) {
       if ((starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t0 + j));
-      before[j] = h, h = fma2(a[j], h, widened(token(xs, j)));
+      before[j] = h, h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
     }
 #pragma unroll
     for (int j = kGlrTokens - 1; j >= 0; --j) {
@@ -116,9 +97,9 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
       if ((ends >> j) & 1) c = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t));
       const bool in_one = t >= span.lo && t < span.hi;
       const Two dh = add2(widened(token(ds, j)), c);
-      c = mul2(a[j], dh);
+      c = mul2(decay_at(decay, j), dh);
       token(ds, j) = narrowed<X>(in_one ? dh : two(0.f));
-      token(gs, j) = narrowed<G>(in_one ? mul2(c, before[j]) : two(0.f));
+      put_gradient<G>(decay, j, in_one ? mul2(c, before[j]) : two(0.f));
       if (p.dh0 != nullptr && in_one && ((starts >> j) & 1))
         store_state<kTma>(p.dh0, s, at, sequence_of(s.seq, at.b, t), c);
     }
@@ -143,7 +124,8 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
 template <typename X, typename G>
 int glr_bwd(const GlrBwdArgs& p, GlrShape s, int x_type, int g_type, bool tma, cudaStream_t stream) {
   const char* what = "linear_recurrence_bwd";
-  const size_t smem = glr_layout<2>(s, 2 * sizeof(X) + sizeof(G), sizeof(G), 3);
+  constexpr size_t smem = kGlrWarps * (kGlrDecays + 2 * kGlrBox<X>);
+  glr_window(s, 3);
   const unsigned grid = unsigned(s.tiles) * s.channel_blocks * s.batch;
   CUtensorMap dy_map{}, x_map{}, g_map{}, dx_map{}, dg_map{};
   if (tma &&

@@ -15,70 +15,58 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
                                                                     const __grid_constant__ CUtensorMap y_map,
                                                                     const GlrFwdArgs p, const GlrShape s) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ GlrShared sh;
+  __shared__ GlrShared<1> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const GlrTileAt at = take_tile<false>(s, sh);
   const int t0 = at.tile * kGlrTile + warp * kGlrTokens;
-  X* xs = reinterpret_cast<X*>(smem + warp * kGlrBox<X>);
-  G* gs = reinterpret_cast<G*>(smem + kGlrWarps * kGlrBox<X> + warp * kGlrBox<G>);
+  float* decay = reinterpret_cast<float*>(smem + warp * kGlrDecays);
+  X* xs = reinterpret_cast<X*>(smem + kGlrWarps * kGlrDecays + warp * kGlrBox<X>);
   bool arrived = true;
   if constexpr (kTma) {
     if (lane == 0) {
       mbar_arrive_expect(&sh.arrived[warp], kGlrBox<X> + kGlrBox<G>);
-      box_load(gs, &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
+      box_load(gates_of<G>(decay), &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(xs, &x_map, at.c0, t0, at.b, &sh.arrived[warp]);
     }
   } else {
-    plain_load(gs, p.g, s, at, t0);
+    plain_load(gates_of<G>(decay), p.g, s, at, t0);
     plain_load(xs, p.x, s, at, t0);
     __syncwarp();
   }
   const Span span = span_of(s.seq, t0);
-  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
   const int n = min(max(s.tokens - t0, 0), kGlrTokens);
   const uint32_t starts = span.bounds & ((1u << n) - 1);
-  Two a[kGlrTokens];
-  to_decays(gs, a);
-  Words tile = fold_tokens<X, kTma>(xs, a, starts, p.h0, s, at, t0);
-  if (!arrived) tile = {kGlrReset, __int_as_float(0x7fffffff), kGlrReset, __int_as_float(0x7fffffff)};
+  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
+  Two A, B, unused;
+  walk_tokens<X, G, false>(decay, xs, xs, A, B, unused);
+  if (starts) fold_from_starts<X, kTma>(decay, xs, starts, p.h0, s, at, t0, A, B);
+  if (!arrived) A = two(kGlrReset), B = two(__int_as_float(0x7fffffff));
+  sh.pair[0][warp][lane] = packed(A, B);
+  __syncthreads();
   Two h = two(0.f);
   if (s.tiles > 1) {
-    const Exchange<1> ex{smem + s.exchange, s.slice};
-    __syncwarp();  // the gates are in registers: their place is free
-    ex.pair(0, warp) = make_float4(tile.A0, tile.B0, tile.A1, tile.B1);
-    __syncthreads();
+    Words tile = words_of(sh.pair[0][0][lane]);
     if (warp == 0) {
 #pragma unroll
-      for (int w = 1; w < kGlrWarps; ++w) chain(tile, ex.pair(0, w));
+      for (int w = 1; w < kGlrWarps; ++w) chain(tile, sh.pair[0][w][lane]);
       publish<kTma>(words_at(p.words, s, at, at.tile), s, at, tile);
     }
-    h = carry_in<kTma, false>(p.words, s, at, sh, ex);
-    if (warp == 0 && !tile.state()) {
-      const float2 in = split(h);
-      publish<kTma>(words_at(p.words, s, at, at.tile), s, at,
-                    Words{kGlrReset, fold(tile.A0, tile.B0, in.x), kGlrReset, fold(tile.A1, tile.B1, in.y)});
-    }
-    for (int w = 0; w < warp; ++w) h = folded(ex.pair(0, w), h);
-  } else {
-    const Exchange<1> ex{smem + s.exchange, s.slice};
-    __syncwarp();
-    ex.pair(0, warp) = make_float4(tile.A0, tile.B0, tile.A1, tile.B1);
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) h = folded(ex.pair(0, w), h);
+    h = carry_in<kTma, false>(p.words, s, at, sh, 0, tile);
   }
+  for (int w = 0; w < warp; ++w) h = folded(sh.pair[0][w][lane], h);
   if (!arrived) h = two(__int_as_float(0x7fffffff));
   if (span.bounds == 0 && t0 >= span.lo && t0 + kGlrTokens <= span.hi) {  // all of one sequence, which goes on
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) {
-      h = fma2(a[j], h, widened(token(xs, j)));
+      h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
       token(xs, j) = narrowed<X>(h);
     }
   } else {
-#pragma unroll
+#pragma unroll 4
     for (int j = 0; j < kGlrTokens; ++j) {
       const int t = t0 + j;
       if ((starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t));
-      h = fma2(a[j], h, widened(token(xs, j)));
+      h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
       const bool in_one = t >= span.lo && t < span.hi;
       token(xs, j) = narrowed<X>(in_one ? h : two(0.f));
       if (p.final_state != nullptr && in_one && span.ends(j))
@@ -103,7 +91,8 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
 template <typename X, typename G>
 int glr_fwd(const GlrFwdArgs& p, GlrShape s, int x_type, int g_type, bool tma, cudaStream_t stream) {
   const char* what = "linear_recurrence_fwd";
-  const size_t smem = glr_layout<1>(s, sizeof(X) + sizeof(G), sizeof(G), 4);
+  constexpr size_t smem = kGlrWarps * (kGlrDecays + kGlrBox<X>);
+  glr_window(s, 4);
   const unsigned grid = unsigned(s.tiles) * s.channel_blocks * s.batch;
   CUtensorMap x_map{}, g_map{}, y_map{};
   if (tma &&
