@@ -370,25 +370,33 @@ __device__ __forceinline__ Two look_back(float* words, const GlrShape& s, const 
 }
 
 // Looking back with the whole block, for chains whose tiles in flight lie far behind one another: warp w looks at the words
-// behind those of warp w - 1 until there is a state with no unset word in front of it; `owner` then folds forward from
-// it, reading the words again (a word that has become a state since gives the same bits).  Only the owner's result counts.
+// behind those of warp w - 1, which it keeps in registers, until there is a state with no unset word in front of it.
+// The fold from there goes forward from warp to warp; the result is in sh.carried.
+constexpr int kGlrWindow = 6;  // words of a warp
 template <bool kPair, bool kReverse, int kDirections>
-__device__ __forceinline__ Two look_back_together(float* words, const GlrShape& s, const GlrTileAt& at,
-                                                  GlrShared<kDirections>& sh, int before, int owner) {
+__device__ __forceinline__ void look_back_together(float* words, const GlrShape& s, const GlrTileAt& at,
+                                                   GlrShared<kDirections>& sh, int before) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float* row = words_at(words, s, at, at.tile);
   const int64_t step = int64_t(kReverse ? 2 : -2) * s.channels;
   constexpr int kFar = 0x7fffffff;
   uint64_t began = 0;
+  Words v[kGlrWindow];
   int from;
   for (;;) {
     int unset = kFar, state = kFar;
-    for (int k = 0; k < s.window; ++k) {
+#pragma unroll
+    for (int k = 0; k < kGlrWindow; ++k) {
       const int back = warp * s.window + k;
-      Words v{kGlrReset, 0.f, kGlrReset, 0.f};  // before the first tile: a state of zero
-      if (back < before) v = load_words<kPair>(row + (back + 1) * step, s, at);
-      if (!__all_sync(0xffffffffu, v.set())) unset = min(unset, back);
-      else if (__all_sync(0xffffffffu, v.state())) state = min(state, back);
+      v[k] = {kGlrReset, 0.f, kGlrReset, 0.f};  // before the first tile: a state of zero
+      if (k < s.window && back < before) v[k] = load_words<kPair>(row + (back + 1) * step, s, at);
+    }
+#pragma unroll
+    for (int k = 0; k < kGlrWindow; ++k) {
+      if (k < s.window) {
+        if (!__all_sync(0xffffffffu, v[k].set())) unset = min(unset, warp * s.window + k);
+        else if (__all_sync(0xffffffffu, v[k].state())) state = min(state, warp * s.window + k);
+      }
     }
     if (lane == 0) sh.marks[warp] = make_int2(unset, state);
     if (threadIdx.x == 0) {
@@ -399,28 +407,30 @@ __device__ __forceinline__ Two look_back_together(float* words, const GlrShape& 
     __syncthreads();
     const int2 mark = sh.marks[lane & (kGlrWarps - 1)];
     unset = __reduce_min_sync(0xffffffffu, mark.x), from = __reduce_min_sync(0xffffffffu, mark.y);
-    const bool late = sh.late != 0;
     if (from < unset) break;
-    if (late) return two(__int_as_float(0x7fffffff));
+    if (sh.late != 0) {
+      sh.carried[lane] = two(__int_as_float(0x7fffffff));  // every warp the same
+      __syncthreads();
+      return;
+    }
     __syncthreads();  // before the marks are set again
   }
   float h[2] = {0.f, 0.f};
-  if (warp == owner) {
-    for (; from >= 0; from -= kGlrNear) {
-      Words v[kGlrNear];
-#pragma unroll
-      for (int k = 0; k < kGlrNear; ++k) {
-        v[k] = {kGlrReset, h[0], kGlrReset, h[1]};
-        const int back = from - k;
-        if (back >= 0 && back < before) v[k] = load_words<kPair>(row + (back + 1) * step, s, at);
-        else if (back >= 0) v[k] = {kGlrReset, 0.f, kGlrReset, 0.f};
+  const int top = from / s.window;
+  for (int w = top; w >= 0; --w) {
+    if (warp == w) {
+      if (w < top) {
+        const float2 f = split(sh.carried[lane]);
+        h[0] = f.x, h[1] = f.y;
       }
 #pragma unroll
-      for (int k = 0; k < kGlrNear; ++k)
-        if (from - k >= 0) h[0] = fold(v[k].A0, v[k].B0, h[0]), h[1] = fold(v[k].A1, v[k].B1, h[1]);
+      for (int k = kGlrWindow - 1; k >= 0; --k)
+        if (k < s.window && w * s.window + k <= from)
+          h[0] = fold(v[k].A0, v[k].B0, h[0]), h[1] = fold(v[k].A1, v[k].B1, h[1]);
+      sh.carried[lane] = two(h[0], h[1]);
     }
+    __syncthreads();
   }
-  return two(h[0], h[1]);
 }
 
 // The state that enters the tile (from the left; reversed: the adjoint from the right), in every warp.  Called by the
@@ -431,18 +441,19 @@ __device__ __forceinline__ Two carry_in(float* words, const GlrShape& s, const G
   const int before = kReverse ? s.tiles - 1 - at.tile : at.tile;  // tiles that come before this one
   const bool mine = int(threadIdx.x >> 5) == owner;
   Two h = two(0.f);
-  if (before > 0) {
-    if (s.window > 0) h = look_back_together<kPair, kReverse>(words, s, at, sh, before, owner);
-    else if (mine) h = look_back<kPair, kReverse>(words, s, at, before);
+  if (before > 0 && s.window > 0) {
+    look_back_together<kPair, kReverse>(words, s, at, sh, before);
+    h = sh.carried[threadIdx.x & 31];
+  } else if (before > 0 && mine) {
+    h = look_back<kPair, kReverse>(words, s, at, before);
   }
-  if (mine) {
-    if (!tile.state()) {  // else it was one already
-      const float2 in = split(h);
-      publish<kPair>(words_at(words, s, at, at.tile), s, at,
-                     Words{kGlrReset, fold(tile.A0, tile.B0, in.x), kGlrReset, fold(tile.A1, tile.B1, in.y)});
-    }
-    sh.carried[threadIdx.x & 31] = h;
+  if (mine && !tile.state()) {  // else it was one already
+    const float2 in = split(h);
+    publish<kPair>(words_at(words, s, at, at.tile), s, at,
+                   Words{kGlrReset, fold(tile.A0, tile.B0, in.x), kGlrReset, fold(tile.A1, tile.B1, in.y)});
   }
+  if (before == 0 || s.window > 0) return h;
+  if (mine) sh.carried[threadIdx.x & 31] = h;
   __syncthreads();
   return sh.carried[threadIdx.x & 31];
 }
@@ -480,10 +491,35 @@ __device__ __forceinline__ void put_gradient(float* decays, int j, Two dg) {
   token(gates_of<G>(decays), j) = narrowed<G>(dg);
 }
 
+// Where sequences start and end among a warp's 16 tokens.
+enum : int { kInside = 0, kOneEdge = 1, kManyEdges = 2 };
+struct Edges {
+  uint32_t starts, ends, live;  // live: tokens of a sequence; the others' outputs are zero and reach no live token
+  int kind;                     // kInside: no boundary, all live; kOneEdge: at most one start and one end
+  int start, end;               // of kOneEdge: their tokens, or -1
+  int start_seq, end_seq;
+  __device__ __forceinline__ Edges(const Sequences& s, const Span& span, int b, int t0) {
+    const int n = min(max(s.tokens - t0, 0), kGlrTokens);
+    auto below = [](int k) { return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1; };
+    const uint32_t here = below(n);
+    live = here & below(span.hi - t0) & ~below(span.lo - t0);
+    starts = span.bounds & live;
+    ends = (span.bounds >> 1) & live;
+    kind = (starts | ends) == 0 && live == below(kGlrTokens) ? kInside
+           : __popc(starts) <= 1 && __popc(ends) <= 1        ? kOneEdge
+                                                             : kManyEdges;
+    start = kind == kOneEdge ? __ffs(starts) - 1 : -1, end = kind == kOneEdge ? __ffs(ends) - 1 : -1;
+    start_seq = start >= 0 ? sequence_of(s, b, t0 + start) : 0;
+    end_seq = end >= 0 ? sequence_of(s, b, t0 + end) : 0;
+  }
+};
+
 // One walk over the warp's tokens: gates to decays, and the fold of the run to (A, B); with gradients ds (kBack) also to
-// (A, D), D the adjoint that leaves the first token to the left when nothing enters at the last.
-template <typename X, typename G, bool kBack>
-__device__ __forceinline__ void walk_tokens(float* decay, X* xs, X* ds, Two& A, Two& B, Two& D) {
+// (A, D), D the adjoint that leaves the first token to the left when nothing enters at the last.  kEdge: a sequence
+// may start at edges.start from the state s0 and end at edges.end with the adjoint d1.
+template <typename X, typename G, bool kBack, bool kEdge>
+__device__ __forceinline__ void walk_tokens(float* decay, X* xs, X* ds, const Edges& edges, Two s0, Two d1, Two& A, Two& B,
+                                            Two& D) {
   G* gates = gates_of<G>(decay);
   A = two(1.f), B = D = two(0.f);
 #pragma unroll
@@ -491,31 +527,36 @@ __device__ __forceinline__ void walk_tokens(float* decay, X* xs, X* ds, Two& A, 
     const Two a = decays(widened(token(gates, j)));
     put_decay<G>(decay, j, a);
     A = mul2(A, a);
+    if (kEdge && j == edges.start) B = s0;
     B = fma2(a, B, widened(token(xs, j)));
-    if constexpr (kBack) D = fma2(A, widened(token(ds, j)), D);
+    if constexpr (kBack) {
+      if (!kEdge || edges.end < 0 || j <= edges.end) D = fma2(A, widened(token(ds, j)), D);
+      if (kEdge && j == edges.end) D = fma2(A, d1, D);
+    }
   }
 }
-// The same folds where sequences start or end among the tokens; a fold that meets a boundary does not depend on what
-// comes before (A < 0).
+// The same folds where sequences start or end more than once among the tokens.
 template <typename X, bool kPair>
-__device__ __forceinline__ void fold_from_starts(const float* decay, X* xs, uint32_t starts, const float* __restrict__ h0,
-                                                 const GlrShape& s, const GlrTileAt& at, int t0, Two& A, Two& B) {
-  B = two(0.f), A = two(kGlrReset);
-#pragma unroll 4
+__device__ __noinline__ Two fold_from_starts(const float* decay, X* xs, uint32_t starts, const float* __restrict__ h0,
+                                             const GlrShape& s, const GlrTileAt& at, int t0) {
+  Two B = two(0.f);
+#pragma unroll 1
   for (int j = 0; j < kGlrTokens; ++j) {
     if ((starts >> j) & 1) B = load_state<kPair>(h0, s, at, sequence_of(s.seq, at.b, t0 + j));
     B = fma2(decay_at(decay, j), B, widened(token(xs, j)));
   }
+  return B;
 }
 template <typename X, bool kPair>
-__device__ __forceinline__ void fold_from_ends(const float* decay, X* ds, uint32_t ends, const float* __restrict__ d_final,
-                                               const GlrShape& s, const GlrTileAt& at, int t0, Two& A, Two& D) {
-  D = two(0.f), A = two(kGlrReset);
-#pragma unroll 4
+__device__ __noinline__ Two fold_from_ends(const float* decay, X* ds, uint32_t ends, const float* __restrict__ d_final,
+                                           const GlrShape& s, const GlrTileAt& at, int t0) {
+  Two D = two(0.f);
+#pragma unroll 1
   for (int j = kGlrTokens - 1; j >= 0; --j) {
     if ((ends >> j) & 1) D = load_state<kPair>(d_final, s, at, sequence_of(s.seq, at.b, t0 + j));
     D = mul2(decay_at(decay, j), add2(widened(token(ds, j)), D));
   }
+  return D;
 }
 __device__ __forceinline__ float4 packed(Two A, Two B) {
   const float2 a = split(A), b = split(B);
@@ -556,7 +597,7 @@ inline GlrShape glr_shape(int64_t batch, int64_t tokens, int64_t channels, int64
 // instructions.
 inline void glr_window(GlrShape& s, int blocks_per_sm) {
   const int64_t chains = int64_t(s.batch) * s.channel_blocks, depth = (blocks_per_sm * 148 + chains - 1) / chains;
-  s.window = int(depth >= 6 * kGlrWarps ? 6 : depth <= kGlrNear ? 0 : (depth + kGlrWarps - 1) / kGlrWarps);
+  s.window = int(depth >= kGlrWindow * kGlrWarps ? kGlrWindow : depth <= kGlrNear ? 0 : (depth + kGlrWarps - 1) / kGlrWarps);
 }
 
 // Words unset and the counter behind them at -1: one asynchronous fill with ones (nothing where a chain is one tile).

@@ -46,16 +46,21 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
     const Words v = load_words<kTma>(words_at(const_cast<float*>(p.states), s, at, at.tile - 1), s, at);
     h = two(v.B0, v.B1);
   }
-  const Span span = span_of(s.seq, t0);
-  const int n = min(max(s.tokens - t0, 0), kGlrTokens);
-  const uint32_t starts = span.bounds & ((1u << n) - 1), ends = (span.bounds >> 1) & ((1u << n) - 1);
+  const Edges edges(s.seq, span_of(s.seq, t0), at.b, t0);
+  const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
+  const Two d1 = edges.end >= 0 ? load_state<kTma>(p.d_final, s, at, edges.end_seq) : two(0.f);
   if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
   {
     Two A, B, D;
-    walk_tokens<X, G, true>(decay, xs, ds, A, B, D);
+    if (edges.kind == kInside) walk_tokens<X, G, true, false>(decay, xs, ds, edges, s0, d1, A, B, D);
+    else walk_tokens<X, G, true, true>(decay, xs, ds, edges, s0, d1, A, B, D);
     Two R = A;
-    if (starts) fold_from_starts<X, kTma>(decay, xs, starts, p.h0, s, at, t0, A, B);
-    if (ends) fold_from_ends<X, kTma>(decay, ds, ends, p.d_final, s, at, t0, R, D);
+    if (edges.kind == kManyEdges) {
+      if (edges.starts) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
+      if (edges.ends) D = fold_from_ends<X, kTma>(decay, ds, edges.ends, p.d_final, s, at, t0);
+    }
+    if (edges.starts) A = two(kGlrReset);
+    if (edges.ends) R = two(kGlrReset);
     if (!arrived) R = two(kGlrReset), D = two(__int_as_float(0x7fffffff));
     sh.pair[0][warp][lane] = packed(A, B);
     sh.pair[1][warp][lane] = packed(R, D);
@@ -75,7 +80,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   if (!arrived) c = two(__int_as_float(0x7fffffff));
   // forward once more for the state before every token, then back with the adjoint; dx takes dy's place, dg the gates'
   Two before[kGlrTokens];
-  if (span.bounds == 0 && t0 >= span.lo && t0 + kGlrTokens <= span.hi) {
+  if (edges.kind == kInside) {
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) before[j] = h, h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
 #pragma unroll
@@ -86,23 +91,28 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
       put_gradient<G>(decay, j, mul2(c, before[j]));
     }
   } else {
+    const bool one = edges.kind == kOneEdge;
+    Two first = two(0.f);
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) {
-      if ((starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t0 + j));
+      if (j == edges.start) h = s0;
+      if (!one && ((edges.starts >> j) & 1)) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t0 + j));
       before[j] = h, h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
     }
 #pragma unroll
     for (int j = kGlrTokens - 1; j >= 0; --j) {
-      const int t = t0 + j;
-      if ((ends >> j) & 1) c = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t));
-      const bool in_one = t >= span.lo && t < span.hi;
+      if (j == edges.end) c = d1;
+      if (!one && ((edges.ends >> j) & 1)) c = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t0 + j));
       const Two dh = add2(widened(token(ds, j)), c);
       c = mul2(decay_at(decay, j), dh);
-      token(ds, j) = narrowed<X>(in_one ? dh : two(0.f));
-      put_gradient<G>(decay, j, in_one ? mul2(c, before[j]) : two(0.f));
-      if (p.dh0 != nullptr && in_one && ((starts >> j) & 1))
-        store_state<kTma>(p.dh0, s, at, sequence_of(s.seq, at.b, t), c);
+      const bool live = (edges.live >> j) & 1;
+      token(ds, j) = narrowed<X>(live ? dh : two(0.f));
+      put_gradient<G>(decay, j, live ? mul2(c, before[j]) : two(0.f));
+      if (j == edges.start) first = c;
+      if (!one && p.dh0 != nullptr && live && ((edges.starts >> j) & 1))
+        store_state<kTma>(p.dh0, s, at, sequence_of(s.seq, at.b, t0 + j), c);
     }
+    if (p.dh0 != nullptr && edges.start >= 0) store_state<kTma>(p.dh0, s, at, edges.start_seq, first);
   }
   if constexpr (kTma) {
     fence_async_smem();

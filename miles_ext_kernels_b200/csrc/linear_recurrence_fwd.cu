@@ -33,13 +33,14 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
     plain_load(xs, p.x, s, at, t0);
     __syncwarp();
   }
-  const Span span = span_of(s.seq, t0);
-  const int n = min(max(s.tokens - t0, 0), kGlrTokens);
-  const uint32_t starts = span.bounds & ((1u << n) - 1);
+  const Edges edges(s.seq, span_of(s.seq, t0), at.b, t0);
+  const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
   if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
-  Two A, B, unused;
-  walk_tokens<X, G, false>(decay, xs, xs, A, B, unused);
-  if (starts) fold_from_starts<X, kTma>(decay, xs, starts, p.h0, s, at, t0, A, B);
+  Two A, B, none;
+  if (edges.kind == kInside) walk_tokens<X, G, false, false>(decay, xs, xs, edges, none, none, A, B, none);
+  else walk_tokens<X, G, false, true>(decay, xs, xs, edges, s0, none, A, B, none);
+  if (edges.kind == kManyEdges) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
+  if (edges.starts) A = two(kGlrReset);
   if (!arrived) A = two(kGlrReset), B = two(__int_as_float(0x7fffffff));
   sh.pair[0][warp][lane] = packed(A, B);
   __syncthreads();
@@ -55,21 +56,31 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   }
   for (int w = 0; w < warp; ++w) h = folded(sh.pair[0][w][lane], h);
   if (!arrived) h = two(__int_as_float(0x7fffffff));
-  if (span.bounds == 0 && t0 >= span.lo && t0 + kGlrTokens <= span.hi) {  // all of one sequence, which goes on
+  if (edges.kind == kInside) {
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) {
       h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
       token(xs, j) = narrowed<X>(h);
     }
+  } else if (edges.kind == kOneEdge) {
+    Two last = two(0.f);
+#pragma unroll
+    for (int j = 0; j < kGlrTokens; ++j) {
+      if (j == edges.start) h = s0;
+      h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
+      if (j == edges.end) last = h;
+      token(xs, j) = narrowed<X>((edges.live >> j) & 1 ? h : two(0.f));
+    }
+    if (p.final_state != nullptr && edges.end >= 0) store_state<kTma>(p.final_state, s, at, edges.end_seq, last);
   } else {
-#pragma unroll 4
+#pragma unroll 1
     for (int j = 0; j < kGlrTokens; ++j) {
       const int t = t0 + j;
-      if ((starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t));
+      if ((edges.starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t));
       h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
-      const bool in_one = t >= span.lo && t < span.hi;
-      token(xs, j) = narrowed<X>(in_one ? h : two(0.f));
-      if (p.final_state != nullptr && in_one && span.ends(j))
+      const bool live = (edges.live >> j) & 1;
+      token(xs, j) = narrowed<X>(live ? h : two(0.f));
+      if (p.final_state != nullptr && live && ((edges.ends >> j) & 1))
         store_state<kTma>(p.final_state, s, at, sequence_of(s.seq, at.b, t), h);
     }
   }
