@@ -34,6 +34,13 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
       box_load(gs, &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(ds, &dy_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(xs, &x_map, at.c0, t0, at.b, &sh.arrived[warp]);
+      const GlrTileAt next = sh.ahead;
+      if (next.tile >= 0) {
+        const int t = next.tile * kGlrTile + warp * kGlrTokens;
+        box_prefetch(&g_map, next.c0, t, next.b);
+        box_prefetch(&dy_map, next.c0, t, next.b);
+        box_prefetch(&x_map, next.c0, t, next.b);
+      }
     }
   } else {
     plain_load(gs, p.g, s, at, t0);
@@ -75,8 +82,12 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
     }
     c = carry_in<kTma, true>(p.words, s, at, sh, kGlrWarps - 1, tile);
   }
-  for (int w = 0; w < warp; ++w) h = folded(sh.pair[0][w][lane], h);
-  for (int w = kGlrWarps - 1; w > warp; --w) c = folded(sh.pair[1][w][lane], c);
+#pragma unroll
+  for (int w = 0; w < kGlrWarps - 1; ++w)
+    if (w < warp) h = folded(sh.pair[0][w][lane], h);
+#pragma unroll
+  for (int w = kGlrWarps - 1; w > 0; --w)
+    if (w > warp) c = folded(sh.pair[1][w][lane], c);
   if (!arrived) c = two(__int_as_float(0x7fffffff));
   // forward once more for the state before every token, then back with the adjoint; dx takes dy's place, dg the gates'
   Two before[kGlrTokens];

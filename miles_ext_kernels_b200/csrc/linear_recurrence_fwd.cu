@@ -27,6 +27,11 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
       mbar_arrive_expect(&sh.arrived[warp], kGlrBox<X> + kGlrBox<G>);
       box_load(gates_of<G>(decay), &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(xs, &x_map, at.c0, t0, at.b, &sh.arrived[warp]);
+      const GlrTileAt next = sh.ahead;
+      if (next.tile >= 0) {
+        box_prefetch(&g_map, next.c0, next.tile * kGlrTile + warp * kGlrTokens, next.b);
+        box_prefetch(&x_map, next.c0, next.tile * kGlrTile + warp * kGlrTokens, next.b);
+      }
     }
   } else {
     plain_load(gates_of<G>(decay), p.g, s, at, t0);
@@ -54,7 +59,9 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
     }
     h = carry_in<kTma, false>(p.words, s, at, sh, 0, tile);
   }
-  for (int w = 0; w < warp; ++w) h = folded(sh.pair[0][w][lane], h);
+#pragma unroll
+  for (int w = 0; w < kGlrWarps - 1; ++w)
+    if (w < warp) h = folded(sh.pair[0][w][lane], h);
   if (!arrived) h = two(__int_as_float(0x7fffffff));
   if (edges.kind == kInside) {
 #pragma unroll
