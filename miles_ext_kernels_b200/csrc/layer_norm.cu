@@ -16,204 +16,418 @@
 
 #include "common.cuh"
 #include "rowio.cuh"
+#include "tma.cuh"
+#include "umma.cuh"
 
 namespace mek {
 
 constexpr int kLnSms = 148;
 
-template <int G>
-struct RowGroup {  // G threads own a row; blocks of one warp's rows hold four
-  static constexpr int kThreads = G < 128 ? 128 : G;
-  static constexpr int kRows = kThreads / G;
-  static constexpr int kWarps = G / 32;
+constexpr int kLnMaxSlots = 8;
+
+// How a group of G threads holds a row: NV accesses of VEC elements a thread, in packed pairs.  Pair q of a thread:
+// neighbouring columns of one access, or (VEC = 1, NV even) the columns of two accesses.
+template <typename T, int VEC, int G, int NV>
+struct RowShape {
+  static constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, kWarps = G / 32, kPairs = NV * VEC / 2;
+  static_assert(NV * VEC % 2 == 0, "pairs");
+  static __device__ __forceinline__ int column(int lane, int q, int i) {
+    if constexpr (VEC == 1) return (2 * q + i) * G + lane;
+    else return (q / (VEC / 2) * G + lane) * VEC + q % (VEC / 2) * 2 + i;
+  }
+  // elements of a row of `width` that warp w of the group holds
+  static __device__ __forceinline__ int count(int w, int width) {
+    int n = 0;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) n += min(max(width - (v * G + w * 32) * VEC, 0), 32 * VEC);
+    return n;
+  }
 };
 
-// x [rows, width] with a row stride; y and codes dense.  grid-stride over rows.
-template <typename T, int VEC, int G, int NV>
-__global__ void __launch_bounds__(RowGroup<G>::kThreads) layer_norm_fwd_kernel(
-    const T* __restrict__ x, int64_t x_stride, const void* __restrict__ weight, const void* __restrict__ bias,
-    int param_type, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
-    uint8_t* __restrict__ codes, int64_t rows, int width, float eps) {
-  constexpr int kRows = RowGroup<G>::kRows, kWarps = RowGroup<G>::kWarps;
-  __shared__ float2 s_part[2][kWarps];
-  const int lane = threadIdx.x % G, warp = lane / 32;
-  float w[NV][VEC], b[NV][VEC];
-  int counts = 0;  // elements of a row this warp owns
+// A thread's part of a row as it lies in memory (zeros past the row's end), and its pairs.
+template <typename E, int VEC, int G, int NV>
+struct RowPart {
+  Vec<E, VEC> raw[NV];
+  __device__ __forceinline__ void load(const E* row, int lane, int width) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * G + lane) * VEC;
+      if (c < width) raw[v] = *reinterpret_cast<const Vec<E, VEC>*>(row + c);
+      else
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) raw[v].e[i] = from_float<E>(0.f);
+    }
+  }
+  __device__ __forceinline__ Two pair(int q) const {
+    Vec<E, 2> two_of;
+    if constexpr (VEC == 1) two_of = {{raw[2 * q].e[0], raw[2 * q + 1].e[0]}};
+    else two_of = {{raw[q / (VEC / 2)].e[q % (VEC / 2) * 2], raw[q / (VEC / 2)].e[q % (VEC / 2) * 2 + 1]}};
+    return widened(two_of);
+  }
+};
+template <int VEC, int G, int NV>
+struct RowPart<uint8_t, VEC, G, NV> {
+  Vec<uint8_t, VEC> raw[NV];
+  __device__ __forceinline__ void load(const uint8_t* row, int lane, int width) {
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      const int c = (v * G + lane) * VEC;
+      if (c < width) raw[v] = *reinterpret_cast<const Vec<uint8_t, VEC>*>(row + c);
+      else
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) raw[v].e[i] = 0;
+    }
+  }
+  __device__ __forceinline__ Two pair(int q) const {
+    Vec<uint8_t, 2> codes;
+    if constexpr (VEC == 1) codes = {{raw[2 * q].e[0], raw[2 * q + 1].e[0]}};
+    else codes = {{raw[q / (VEC / 2)].e[q % (VEC / 2) * 2], raw[q / (VEC / 2)].e[q % (VEC / 2) * 2 + 1]}};
+    float f[2];
+    from_e4m3(codes, f);
+    return two(f[0], f[1]);
+  }
+};
+template <typename E, int VEC, int G, int NV, typename Value>  // value(q) -> Two
+__device__ __forceinline__ void store_row(E* row, int lane, int width, Value value) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = (v * G + lane) * VEC;
-    counts += min(max(width - (v * G + warp * 32) * VEC, 0), 32 * VEC);
+    if constexpr (VEC == 1) {
+      if (v % 2) continue;
+      const float2 f = split(value(v / 2));
+      if (c < width) row[c] = from_float<E>(f.x);
+      if (c + G < width) row[c + G] = from_float<E>(f.y);
+    } else {
+      if (c >= width) continue;
+      float f[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const bool in = c + i < width;
-      w[v][i] = in && weight ? load_param(weight, param_type, c + i) : 1.f;
-      b[v][i] = in && bias ? load_param(bias, param_type, c + i) : 0.f;
+      for (int i = 0; i < VEC / 2; ++i) {
+        const float2 p = split(value(v * (VEC / 2) + i));
+        f[2 * i] = p.x, f[2 * i + 1] = p.y;
+      }
+      *reinterpret_cast<Vec<E, VEC>*>(row + c) = pack<E, VEC>(f);
     }
   }
-  const float inv_count = counts ? 1.f / float(counts) : 0.f, inv_width = 1.f / float(width);
-  int phase = 0;
-  for (int64_t r0 = int64_t(blockIdx.x) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * kRows) {
-    const int64_t r = r0 + threadIdx.x / G;
-    const bool live = r < rows;  // uniform over a group; groups share barriers only when a block is one group
-    float xv[NV][VEC];
-    float sum = 0.f;
+}
+template <int VEC, int G, int NV, typename Value>
+__device__ __forceinline__ void store_codes(uint8_t* row, int lane, int width, Value value) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + lane) * VEC;
-      if (live && c < width) unpack(*reinterpret_cast<const Vec<T, VEC>*>(x + r * x_stride + c), xv[v]);
-      else
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) xv[v][i] = 0.f;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) sum += xv[v][i];
-    }
-    // of this warp's elements; rounded before it is subtracted, whether or not it is stored: the same y either way
-    float mean = __fmul_rn(warp_sum(sum), inv_count), m2 = 0.f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-      if ((v * G + lane) * VEC < width)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) m2 = fmaf(xv[v][i] - mean, xv[v][i] - mean, m2);
-    m2 = warp_sum(m2);
-    if constexpr (kWarps > 1) {
-      if (threadIdx.x % 32 == 0) s_part[phase][warp] = make_float2(mean, m2);
-      __syncthreads();
-      float total = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        int n = 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) n += min(max(width - (v * G + k * 32) * VEC, 0), 32 * VEC);
-        total = fmaf(float(n), s_part[phase][k].x, total);
-      }
-      mean = __fmul_rn(total, inv_width);
-      m2 = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        int n = 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v) n += min(max(width - (v * G + k * 32) * VEC, 0), 32 * VEC);
-        const float d = s_part[phase][k].x - mean;
-        m2 += fmaf(float(n) * d, d, s_part[phase][k].y);
-      }
-      phase ^= 1;  // the other half: a slow warp may still read this one
-    }
-    const float rstd = rsqrtf(m2 * inv_width + eps);
-    if (!live) continue;
-    if (lane == 0) {
-      if (mean_out) mean_out[r] = mean;
-      if (rstd_out) rstd_out[r] = rstd;
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + lane) * VEC;
+  for (int v = 0; v < NV; ++v) {
+    const int c = (v * G + lane) * VEC;
+    if constexpr (VEC == 1) {
+      if (v % 2) continue;
+      const float2 f = split(value(v / 2));
+      const float a[1] = {f.x}, b[1] = {f.y};
+      if (c < width) row[c] = to_e4m3(a).e[0];
+      if (c + G < width) row[c + G] = to_e4m3(b).e[0];
+    } else {
       if (c >= width) continue;
-      float unit[VEC], out[VEC];
+      float f[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        unit[i] = (xv[v][i] - mean) * rstd;
-        out[i] = fmaf(unit[i], w[v][i], b[v][i]);
+      for (int i = 0; i < VEC / 2; ++i) {
+        const float2 p = split(value(v * (VEC / 2) + i));
+        f[2 * i] = p.x, f[2 * i + 1] = p.y;
       }
-      *reinterpret_cast<Vec<T, VEC>*>(y + r * width + c) = pack<T, VEC>(out);
-      if (codes) *reinterpret_cast<Vec<uint8_t, VEC>*>(codes + r * width + c) = to_e4m3(unit);
+      *reinterpret_cast<Vec<uint8_t, VEC>*>(row + c) = to_e4m3(f);
     }
   }
 }
 
-// kCodes: unit comes from the 8-bit checkpoint, x and mean are not read.  partial [gridDim.x, 2, width] (or NULL).
-template <typename T, int VEC, int G, int NV, bool kCodes>
-__global__ void __launch_bounds__(RowGroup<G>::kThreads) layer_norm_bwd_kernel(
-    const T* __restrict__ dy, const T* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ codes,
-    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const void* __restrict__ weight,
-    int param_type, T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width) {
-  constexpr int kRows = RowGroup<G>::kRows, kWarps = RowGroup<G>::kWarps;
-  __shared__ float2 s_part[2][kWarps];
-  const int lane = threadIdx.x % G, warp = lane / 32;
-  float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+// Sums over a group of two values, the warps' sums through shared memory (`phase` alternates: one barrier a row).
+template <int G>
+__device__ __forceinline__ float2 group_sum(float a, float b, float2 (*part)[32], int phase) {
+  a = warp_sum(a), b = warp_sum(b);
+  if constexpr (G == 32) return make_float2(a, b);
+  if (threadIdx.x % 32 == 0) part[phase][threadIdx.x / 32] = make_float2(a, b);
+  __syncthreads();
+  if constexpr (G <= 256) {
+    a = b = 0.f;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+    for (int w = 0; w < G / 32; ++w) a += part[phase][w].x, b += part[phase][w].y;
+    return make_float2(a, b);
+  } else {
+    const float2 p = threadIdx.x % 32 < G / 32 ? part[phase][threadIdx.x % 32] : make_float2(0.f, 0.f);
+    return make_float2(warp_sum(p.x), warp_sum(p.y));
+  }
+}
+
+// Where a block's rows come from.  Rows of wide accesses that take a whole block are streamed through shared memory: one
+// thread asks for the next rows with bulk copies, `slots` rows ahead, so the loads in flight depend neither on registers
+// nor on how far the block is inside a row.  Other rows are loaded a row ahead into registers.
+__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(to)),
+               "l"(from), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+template <int VEC, int G>
+constexpr bool kLnStreams = VEC > 1 && G >= 128;
+template <int G>
+constexpr int kLnBlocks = G <= 128 ? 6 : G == 256 ? 3 : 1;  // blocks an SM, for about 80 registers a thread (1,024: 64)
+// Groups of 1,024 threads have 64 registers: their parameters stay in shared memory.
+template <int G>
+constexpr bool kLnParamsShared = G == 1024;
+
+// The parameters of a thread's columns, FP32.
+template <typename T, int VEC, int G, int NV>
+struct RowParams {
+  typedef RowShape<T, VEC, G, NV> Shape;
+  Two kept[kLnParamsShared<G> ? 1 : Shape::kPairs];
+  const float* shared;
+  int last;  // columns past the row's end read its last parameters, and nobody what comes of it
+  __device__ __forceinline__ void load(const void* p, int type, float missing, float* room, int lane, int width) {
+    shared = room, last = VEC == 1 ? width - 1 : width - 2;
+    if constexpr (kLnParamsShared<G>) {
+      for (int c = lane; c < width; c += G) room[c] = p ? load_param(p, type, c) : missing;
+    } else {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int c = (v * G + lane) * VEC + i;
-      w[v][i] = c < width && weight ? load_param(weight, param_type, c) : 1.f;
-      dw[v][i] = db[v][i] = 0.f;
-    }
-  const float inv_width = 1.f / float(width);
-  int phase = 0;
-  for (int64_t r0 = int64_t(blockIdx.x) * kRows; r0 < rows; r0 += int64_t(gridDim.x) * kRows) {
-    const int64_t r = r0 + threadIdx.x / G;
-    const bool live = r < rows;
-    const float rstd = live ? rstd_in[r] : 0.f, mean = live && !kCodes ? mean_in[r] : 0.f;
-    float unit[NV][VEC], dn[NV][VEC];
-    float s1 = 0.f, s2 = 0.f;
+      for (int q = 0; q < Shape::kPairs; ++q) {
+        float f[2];
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + lane) * VEC;
-      if (live && c < width) {
-        if constexpr (kCodes) {
-          from_e4m3(*reinterpret_cast<const Vec<uint8_t, VEC>*>(codes + r * width + c), unit[v]);
-        } else {
-          unpack(*reinterpret_cast<const Vec<T, VEC>*>(x + r * x_stride + c), unit[v]);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) unit[v][i] = (unit[v][i] - mean) * rstd;
+        for (int i = 0; i < 2; ++i) {
+          const int c = Shape::column(lane, q, i);
+          f[i] = p && c < width ? load_param(p, type, c) : missing;
         }
-        unpack(*reinterpret_cast<const Vec<T, VEC>*>(dy + r * width + c), dn[v]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          dw[v][i] = fmaf(dn[v][i], unit[v][i], dw[v][i]);
-          db[v][i] += dn[v][i];
-          dn[v][i] *= w[v][i];
-          s1 += dn[v][i];
-          s2 = fmaf(dn[v][i], unit[v][i], s2);
-        }
+        kept[q] = two(f[0], f[1]);
       }
     }
-    s1 = warp_sum(s1), s2 = warp_sum(s2);
-    if constexpr (kWarps > 1) {
-      if (threadIdx.x % 32 == 0) s_part[phase][warp] = make_float2(s1, s2);
+  }
+  __device__ __forceinline__ Two pair(int q, int lane) const {
+    if constexpr (!kLnParamsShared<G>) return kept[q];
+    else if constexpr (VEC == 1)
+      return two(shared[min(Shape::column(lane, q, 0), last)], shared[min(Shape::column(lane, q, 1), last)]);
+    else return *reinterpret_cast<const Two*>(shared + min(Shape::column(lane, q, 0), last));
+  }
+};
+
+// x [rows, width] with a row stride; y and codes dense.  Block b takes rows (or groups of rows) b, b + gridDim.x, ...
+template <typename T, int VEC, int G, int NV>
+__global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G>) layer_norm_fwd_kernel(
+    const T* __restrict__ x, int64_t x_stride, const void* __restrict__ weight, const void* __restrict__ bias,
+    int param_type, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
+    uint8_t* __restrict__ codes, int64_t rows, int width, float eps, int slots) {
+  typedef RowShape<T, VEC, G, NV> Shape;
+  constexpr bool kStream = kLnStreams<VEC, G>;
+  constexpr int kPairs = Shape::kPairs;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 s_part[2][32];
+  __shared__ float s_count[32];
+  __shared__ uint64_t s_full[kLnMaxSlots];
+  const int lane = threadIdx.x % G, warp = lane / 32;
+  const uint32_t bytes = uint32_t(width) * sizeof(T);
+  const int64_t first = int64_t(blockIdx.x) * Shape::kRows + threadIdx.x / G, step = int64_t(gridDim.x) * Shape::kRows;
+  if (kStream && threadIdx.x == 0) {
+    for (int k = 0; k < slots; ++k) mbar_init(&s_full[k], 1);
+    fence_mbar_init();
+    for (int k = 0; k < slots && first + k * step < rows; ++k) {
+      mbar_arrive_expect(&s_full[k], bytes);
+      bulk_load(smem + k * bytes, x + (first + k * step) * x_stride, bytes, &s_full[k]);
+    }
+  }
+  float* room = reinterpret_cast<float*>(smem + size_t(kStream ? slots : 0) * bytes);
+  RowParams<T, VEC, G, NV> w, b;
+  w.load(weight, param_type, 1.f, room, lane, width);
+  b.load(bias, param_type, 0.f, room + width, lane, width);
+  if (threadIdx.x < Shape::kWarps) s_count[threadIdx.x] = float(Shape::count(threadIdx.x, width));
+  const int count = Shape::count(warp, width);
+  const float inv_count = count ? 1.f / float(count) : 0.f, inv_width = 1.f / float(width);
+  const bool full = Shape::column(lane, kPairs - 1, 1) < width;  // no column past the row's end
+  RowPart<T, VEC, G, NV> part;
+  if (!kStream && first < rows) part.load(x + first * x_stride, lane, width);
+  __syncthreads();
+  int slot = 0, parity = 0, phase = 0;
+  for (int64_t r = first; r < rows; r += step, phase ^= 1) {
+    bool arrived = true;
+    if constexpr (kStream) {
+      arrived = mbar_wait_soon(&s_full[slot], parity);
+      part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
+    }
+    Two xv[kPairs], sum = two(0.f);
+#pragma unroll
+    for (int q = 0; q < kPairs; ++q) xv[q] = part.pair(q), sum = add2(sum, xv[q]);
+    if constexpr (!kStream)
+      if (r + step < rows) part.load(x + (r + step) * x_stride, lane, width);
+    // this warp's mean and squares about it; a mean is rounded before it is subtracted, whether or not it is stored: the
+    // same y either way
+    float2 s = split(sum);
+    if (!arrived) s.x = __int_as_float(0x7fffffff);
+    float total = warp_sum(s.x + s.y);
+    float mean = __fmul_rn(total, inv_count);
+    Two squares = two(0.f);
+    const Two mean2 = two(mean);
+    if (full) {
+#pragma unroll
+      for (int q = 0; q < kPairs; ++q) {
+        const Two d = sub2(xv[q], mean2);
+        squares = fma2(d, d, squares);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kPairs; ++q) {
+        const float2 d = split(sub2(xv[q], mean2));
+        const Two in = two(Shape::column(lane, q, 0) < width ? d.x : 0.f, Shape::column(lane, q, 1) < width ? d.y : 0.f);
+        squares = fma2(in, in, squares);
+      }
+    }
+    s = split(squares);
+    float m2 = warp_sum(s.x + s.y);
+    if constexpr (G > 32) {  // the warps' by Chan's rule
+      if (threadIdx.x % 32 == 0) s_part[phase][warp] = make_float2(mean, m2);
       __syncthreads();
-      s1 = s2 = 0.f;
+      if (kStream && threadIdx.x == 0 && r + slots * step < rows) {  // everybody has the row in registers
+        mbar_arrive_expect(&s_full[slot], bytes);
+        bulk_load(smem + slot * bytes, x + (r + slots * step) * x_stride, bytes, &s_full[slot]);
+      }
+      if constexpr (G <= 256) {
+        total = m2 = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) s1 += s_part[phase][k].x, s2 += s_part[phase][k].y;
-      phase ^= 1;
+        for (int k = 0; k < Shape::kWarps; ++k) total = fmaf(s_part[phase][k].x, s_count[k], total);
+        mean = __fmul_rn(total, inv_width);
+#pragma unroll
+        for (int k = 0; k < Shape::kWarps; ++k) {
+          const float d = s_part[phase][k].x - mean;
+          m2 += fmaf(s_count[k] * d, d, s_part[phase][k].y);
+        }
+      } else {
+        const bool in = threadIdx.x % 32 < Shape::kWarps;
+        const float2 p = in ? s_part[phase][threadIdx.x % 32] : make_float2(0.f, 0.f);
+        const float n = in ? s_count[threadIdx.x % 32] : 0.f;
+        mean = __fmul_rn(warp_sum(p.x * n), inv_width);
+        const float d = p.x - mean;
+        m2 = warp_sum(fmaf(n * d, d, p.y));
+      }
     }
-    if (!live) continue;
-    s1 *= inv_width, s2 *= inv_width;
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      const int c = (v * G + lane) * VEC;
-      if (c >= width) continue;
-      float out[VEC];
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out[i] = rstd * (dn[v][i] - s1 - unit[v][i] * s2);
-      *reinterpret_cast<Vec<T, VEC>*>(dx + r * width + c) = pack<T, VEC>(out);
+    const float rstd = rsqrtf(m2 * inv_width + eps);
+    if (lane == 0) {
+      if (mean_out) mean_out[r] = mean;
+      if (rstd_out) rstd_out[r] = rstd;
     }
+    const Two m = two(mean), scale = two(rstd);
+#pragma unroll
+    for (int q = 0; q < kPairs; ++q) xv[q] = mul2(sub2(xv[q], m), scale);  // unit
+    store_row<T, VEC, G, NV>(y + r * width, lane, width, [&](int q) { return fma2(xv[q], w.pair(q, lane), b.pair(q, lane)); });
+    if (codes) store_codes<VEC, G, NV>(codes + r * width, lane, width, [&](int q) { return xv[q]; });
+    if (kStream && ++slot == slots) slot = 0, parity ^= 1;
+  }
+}
+
+// kCodes: unit comes from the 8-bit checkpoint, x and mean are not read.  partial [gridDim.x, 2, width] (or NULL).
+// A streamed row is read from shared memory twice, for the sums and for dx (its slot is filled again once the block has
+// passed the next row's barrier); a row in registers stays there.
+template <typename T, int VEC, int G, int NV, bool kCodes, bool kStream>
+__global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G>) layer_norm_bwd_kernel(
+    const T* __restrict__ dy, const T* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ codes,
+    const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const void* __restrict__ weight,
+    int param_type, T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width, int slots) {
+  typedef RowShape<T, VEC, G, NV> Shape;
+  typedef typename std::conditional<kCodes, uint8_t, T>::type Kept;
+  constexpr int kPairs = Shape::kPairs;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 s_part[2][32];
+  __shared__ uint64_t s_full[kLnMaxSlots];
+  const int lane = threadIdx.x % G;
+  const uint32_t dy_bytes = uint32_t(width) * sizeof(T), kept_bytes = uint32_t(width) * sizeof(Kept);
+  const uint32_t bytes = dy_bytes + kept_bytes;
+  const int64_t first = int64_t(blockIdx.x) * Shape::kRows + threadIdx.x / G, step = int64_t(gridDim.x) * Shape::kRows;
+  auto kept_row = [&](int64_t r) -> const Kept* {
+    if constexpr (kCodes) return codes + r * width;
+    else return x + r * x_stride;
+  };
+  auto fill = [&](int slot, int64_t r) {
+    uint8_t* to = smem + slot * bytes;
+    mbar_arrive_expect(&s_full[slot], bytes);
+    bulk_load(to, dy + r * width, dy_bytes, &s_full[slot]);
+    bulk_load(to + dy_bytes, kept_row(r), kept_bytes, &s_full[slot]);
+  };
+  if (kStream && threadIdx.x == 0) {
+    for (int k = 0; k < slots; ++k) mbar_init(&s_full[k], 1);
+    fence_mbar_init();
+    for (int k = 0; k < slots && first + k * step < rows; ++k) fill(k, first + k * step);
+  }
+  RowParams<T, VEC, G, NV> w;
+  w.load(weight, param_type, 1.f, reinterpret_cast<float*>(smem + size_t(kStream ? slots : 0) * bytes), lane, width);
+  Two dw[kPairs], db[kPairs];
+#pragma unroll
+  for (int q = 0; q < kPairs; ++q) dw[q] = db[q] = two(0.f);
+  const float inv_width = 1.f / float(width);
+  float next_rstd = 0.f, next_mean = 0.f;  // the statistics are a row ahead
+  RowPart<T, VEC, G, NV> g_next;
+  RowPart<Kept, VEC, G, NV> k_next;
+  auto ahead = [&](int64_t r) {
+    if (r >= rows) return;
+    next_rstd = rstd_in[r];
+    if constexpr (!kCodes) next_mean = mean_in[r];
+    if constexpr (!kStream) g_next.load(dy + r * width, lane, width), k_next.load(kept_row(r), lane, width);
+  };
+  ahead(first);
+  __syncthreads();
+  int slot = 0, parity = 0, phase = 0, before = -1;
+  for (int64_t r = first; r < rows; r += step, phase ^= 1) {
+    const float rstd = next_rstd;
+    const Two mean = two(next_mean), scale = two(rstd);
+    bool arrived = true;
+    RowPart<T, VEC, G, NV> g_part;
+    RowPart<Kept, VEC, G, NV> k_part;
+    const T* g_row = reinterpret_cast<const T*>(smem + slot * bytes);
+    const Kept* k_row = reinterpret_cast<const Kept*>(smem + slot * bytes + dy_bytes);
+    if constexpr (kStream) {
+      arrived = mbar_wait_soon(&s_full[slot], parity);
+      g_part.load(g_row, lane, width), k_part.load(k_row, lane, width);
+    } else {
+      g_part = g_next, k_part = k_next;
+    }
+    ahead(r + step);
+    auto unit = [&](int q) {
+      const Two v = k_part.pair(q);
+      if constexpr (kCodes) return v;
+      else return mul2(sub2(v, mean), scale);
+    };
+    Two s1 = two(0.f), s2 = two(0.f);
+#pragma unroll
+    for (int q = 0; q < kPairs; ++q) {  // past the row's end dy is zero
+      const Two u = unit(q), g = g_part.pair(q), dn = mul2(g, w.pair(q, lane));
+      dw[q] = fma2(g, u, dw[q]);
+      db[q] = add2(db[q], g);
+      s1 = add2(s1, dn);
+      s2 = fma2(dn, u, s2);
+    }
+    const float2 a = split(s1), c = split(s2);
+    const float2 sums = group_sum<G>(arrived ? a.x + a.y : __int_as_float(0x7fffffff), c.x + c.y, s_part, phase);
+    if constexpr (kStream) {
+      if (threadIdx.x == 0 && before >= 0 && r + (slots - 1) * step < rows) fill(before, r + (slots - 1) * step);
+      g_part.load(g_row, lane, width), k_part.load(k_row, lane, width);
+    }
+    const Two m1 = two(sums.x * inv_width), m2 = two(-(sums.y * inv_width));
+    store_row<T, VEC, G, NV>(dx + r * width, lane, width, [&](int q) {
+      return mul2(fma2(unit(q), m2, sub2(mul2(g_part.pair(q), w.pair(q, lane)), m1)), scale);
+    });
+    before = slot;
+    if (kStream && ++slot == slots) slot = 0, parity ^= 1;
   }
   if (partial == nullptr) return;
   float* mine = partial + int64_t(blockIdx.x) * 2 * width;
-  if constexpr (kRows == 1) {
+  if constexpr (Shape::kRows == 1) {
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = (v * G + lane) * VEC + i;
-        if (c < width) mine[c] = dw[v][i], mine[width + c] = db[v][i];
-      }
+    for (int q = 0; q < kPairs; ++q) {
+      const float2 a = split(dw[q]), c = split(db[q]);
+      const int c0 = Shape::column(lane, q, 0), c1 = Shape::column(lane, q, 1);
+      if (c0 < width) mine[c0] = a.x, mine[width + c0] = c.x;
+      if (c1 < width) mine[c1] = a.y, mine[width + c1] = c.y;
+    }
   } else {  // the block's groups in order
-    __shared__ float s_cols[kRows][2][G * NV * VEC];
+    __shared__ float s_cols[Shape::kRows][2][G * NV * VEC];
     const int group = threadIdx.x / G;
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const int c = (v * G + lane) * VEC + i;
-        s_cols[group][0][c] = dw[v][i], s_cols[group][1][c] = db[v][i];
-      }
+    for (int q = 0; q < kPairs; ++q) {
+      const float2 a = split(dw[q]), c = split(db[q]);
+      const int c0 = Shape::column(lane, q, 0), c1 = Shape::column(lane, q, 1);
+      s_cols[group][0][c0] = a.x, s_cols[group][1][c0] = c.x;
+      s_cols[group][0][c1] = a.y, s_cols[group][1][c1] = c.y;
+    }
     __syncthreads();
-    for (int c = threadIdx.x; c < width; c += RowGroup<G>::kThreads) {
+    for (int c = threadIdx.x; c < width; c += Shape::kThreads) {
       float a = 0.f, d = 0.f;
 #pragma unroll
-      for (int k = 0; k < kRows; ++k) a += s_cols[k][0][c], d += s_cols[k][1][c];
+      for (int k = 0; k < Shape::kRows; ++k) a += s_cols[k][0][c], d += s_cols[k][1][c];
       mine[c] = a, mine[width + c] = d;
     }
   }
@@ -342,55 +556,76 @@ using namespace mek;
 
 struct LnPlan {
   int vec, group, nv;  // group = 0: the wide kernels
-  int grid;            // blocks of the backward (= rows of the partial sums)
+  int grid, slots;     // slots > 0: the rows are streamed
 };
 
 // vec: elements per access, 16 bytes where every row starts on a 16-byte boundary, else one.  The smallest group
-// of threads that holds a row in at most 16 elements a thread where accesses are wide, 8 where they are not.
-LnPlan ln_plan(int64_t rows, int width, int type, bool aligned) {
-  const int wide = type == kTypeFp32 ? 4 : 8;
-  LnPlan p{aligned ? wide : 1, 0, 0, 0};
+// of threads that holds a row in at most 16 elements a thread where accesses are wide, 8 (at last 16) where they are
+// not.  A row of wide accesses that takes a whole block is streamed (kept_size: bytes an element of what the backward
+// reads besides dy, 0 for the forward): as many rows in flight as 160 KB an SM hold, two to eight.
+LnPlan ln_plan(int64_t rows, int width, int type, bool aligned, int kept_size) {
+  const int size = type == kTypeFp32 ? 4 : 2;
+  LnPlan p{aligned ? 16 / size : 1, 0, 0, 0, 0};
   static const int groups[] = {32, 128, 256, 512, 1024};
-  const int most = p.vec > 1 ? 16 / p.vec : 8;
   for (int g : groups) {
-    if (g * p.vec * most < width && !(g == 1024 && g * p.vec * 2 * most >= width)) continue;
+    const int most = p.vec > 1 ? 16 / p.vec : g == 1024 ? 16 : 8;
+    if (g * p.vec * most < width) continue;
     p.group = g;
-    p.nv = 1;
+    p.nv = p.vec == 1 ? 2 : 1;
     while (g * p.vec * p.nv < width) p.nv *= 2;
     break;
   }
-  const int per_sm = p.group == 0 ? 2 : p.group <= 128 ? 8 : 1024 / p.group;
-  const int64_t blocks = p.group == 32 ? (rows + 3) / 4 : rows;
-  p.grid = int(blocks < kLnSms * per_sm ? blocks : kLnSms * per_sm);
+  int blocks = p.group == 0 ? 2 : p.group <= 128 ? kLnBlocks<128> : p.group == 256 ? kLnBlocks<256> : kLnBlocks<512>;
+  if (p.vec > 1 && p.group >= 128 && (kept_size != 1 || width % 16 == 0)) {  // bulk copies move multiples of 16 bytes
+    const int64_t bytes = int64_t(width) * (size + kept_size), params = p.group == 1024 ? width * (kept_size ? 4 : 8) : 0;
+    const int64_t fit = ((p.group == 1024 ? 210 << 10 : 160 << 10) - params) / (blocks * bytes);
+    p.slots = int(fit > kLnMaxSlots ? kLnMaxSlots : fit);
+    if (p.slots < 2) p.group = p.slots = 0, blocks = 2;
+  }
+  const int64_t most_blocks = p.group == 32 ? (rows + 3) / 4 : rows;
+  p.grid = int(most_blocks < kLnSms * blocks ? most_blocks : kLnSms * blocks);
   return p;
 }
 
 template <typename T, int VEC, int G, int NV>
 int ln_fwd(const LnPlan& p, const void* x, int64_t xs, const void* w, const void* b, int pt, void* y, float* mean,
            float* rstd, uint8_t* codes, int64_t rows, int width, float eps, cudaStream_t s) {
-  layer_norm_fwd_kernel<T, VEC, G, NV><<<p.grid, RowGroup<G>::kThreads, 0, s>>>(
-      static_cast<const T*>(x), xs, w, b, pt, static_cast<T*>(y), mean, rstd, codes, rows, width, eps);
+  const size_t smem = size_t(p.slots) * width * sizeof(T) + (kLnParamsShared<G> ? size_t(width) * 8 : 0);
+  if (smem > 40 << 10)  // with the static part it may pass the 48 KB a launch has without asking
+    if (int rc = want_smem(layer_norm_fwd_kernel<T, VEC, G, NV>, smem, "layer_norm_fwd")) return rc;
+  layer_norm_fwd_kernel<T, VEC, G, NV><<<p.grid, RowShape<T, VEC, G, NV>::kThreads, smem, s>>>(
+      static_cast<const T*>(x), xs, w, b, pt, static_cast<T*>(y), mean, rstd, codes, rows, width, eps, p.slots);
   return launched("layer_norm_fwd");
+}
+template <typename T, int VEC, int G, int NV, bool kCodes, bool kStream>
+int ln_bwd_of(const LnPlan& p, const void* dy, const void* x, int64_t xs, const uint8_t* codes, const float* mean,
+              const float* rstd, const void* w, int pt, void* dx, float* partial, int64_t rows, int width, cudaStream_t s) {
+  const size_t row = size_t(width) * (sizeof(T) + (kCodes ? 1 : sizeof(T)));
+  const size_t smem = p.slots * row + (kLnParamsShared<G> ? size_t(width) * 4 : 0);
+  if (smem > 40 << 10)
+    if (int rc = want_smem(layer_norm_bwd_kernel<T, VEC, G, NV, kCodes, kStream>, smem, "layer_norm_bwd")) return rc;
+  layer_norm_bwd_kernel<T, VEC, G, NV, kCodes, kStream><<<p.grid, RowShape<T, VEC, G, NV>::kThreads, smem, s>>>(
+      static_cast<const T*>(dy), static_cast<const T*>(x), xs, codes, mean, rstd, w, pt, static_cast<T*>(dx), partial, rows,
+      width, p.slots);
+  return launched("layer_norm_bwd");
 }
 template <typename T, int VEC, int G, int NV>
 int ln_bwd(const LnPlan& p, const void* dy, const void* x, int64_t xs, const uint8_t* codes, const float* mean,
            const float* rstd, const void* w, int pt, void* dx, float* partial, int64_t rows, int width,
            cudaStream_t s) {
-  if (codes)
-    layer_norm_bwd_kernel<T, VEC, G, NV, true><<<p.grid, RowGroup<G>::kThreads, 0, s>>>(
-        static_cast<const T*>(dy), nullptr, 0, codes, mean, rstd, w, pt, static_cast<T*>(dx), partial, rows, width);
-  else
-    layer_norm_bwd_kernel<T, VEC, G, NV, false><<<p.grid, RowGroup<G>::kThreads, 0, s>>>(
-        static_cast<const T*>(dy), static_cast<const T*>(x), xs, nullptr, mean, rstd, w, pt, static_cast<T*>(dx),
-        partial, rows, width);
-  return launched("layer_norm_bwd");
+#define MEK_LN_OF(CODES, STREAM) \
+  ln_bwd_of<T, VEC, G, NV, CODES, STREAM>(p, dy, x, xs, codes, mean, rstd, w, pt, dx, partial, rows, width, s)
+  constexpr bool kStream = kLnStreams<VEC, G>;
+  if (!codes) return MEK_LN_OF(false, kStream);
+  if (kStream && p.slots == 0) return MEK_LN_OF(true, false);  // rows of codes that bulk copies cannot move
+  return MEK_LN_OF(true, kStream);
+#undef MEK_LN_OF
 }
 
 // One case per (group, vectors a thread) the plan can give for VEC.
 #define MEK_LN_SHAPES(T, VEC, CALL)                                                          \
   do {                                                                                       \
     if constexpr (VEC == 1) {                                                                \
-      if (p.group == 32 && p.nv == 1) return CALL(T, 1, 32, 1);                              \
       if (p.group == 32 && p.nv == 2) return CALL(T, 1, 32, 2);                              \
       if (p.group == 32 && p.nv == 4) return CALL(T, 1, 32, 4);                              \
       if (p.group == 32 && p.nv == 8) return CALL(T, 1, 32, 8);                              \
@@ -404,14 +639,16 @@ int ln_bwd(const LnPlan& p, const void* dy, const void* x, int64_t xs, const uin
       constexpr int kMost = 16 / VEC;                                                        \
       if (p.group == 32 && p.nv == 1) return CALL(T, VEC, 32, 1);                            \
       if (p.group == 32 && p.nv == 2) return CALL(T, VEC, 32, 2);                            \
-      if (p.group == 32 && p.nv == 4) return CALL(T, VEC, 32, 4);                            \
-      if (p.group == 128 && p.nv == 1) return CALL(T, VEC, 128, 1);                          \
       if (p.group == 128 && p.nv == 2) return CALL(T, VEC, 128, 2);                          \
-      if (p.group == 128 && p.nv == 4) return CALL(T, VEC, 128, 4);                          \
+      if constexpr (VEC == 4) {                                                              \
+        if (p.group == 32 && p.nv == 4) return CALL(T, VEC, 32, 4);                          \
+        if (p.group == 128 && p.nv == 4) return CALL(T, VEC, 128, 4);                        \
+      } else {                                                                               \
+        if (p.group == 128 && p.nv == 1) return CALL(T, VEC, 128, 1);                        \
+      }                                                                                      \
       if (p.group == 256 && p.nv == kMost) return CALL(T, VEC, 256, kMost);                  \
       if (p.group == 512 && p.nv == kMost) return CALL(T, VEC, 512, kMost);                  \
       if (p.group == 1024 && p.nv == kMost) return CALL(T, VEC, 1024, kMost);                \
-      if (p.group == 1024 && p.nv == 2 * kMost) return CALL(T, VEC, 1024, 2 * kMost);        \
     }                                                                                        \
   } while (0)
 
@@ -437,8 +674,13 @@ extern "C" {
 
 int mek_layer_norm_partial_rows(int64_t rows, int64_t width, int type) {
   if (rows <= 0 || width <= 0 || width > (1 << 24)) return 0;
-  const LnPlan a = ln_plan(rows, int(width), type, true), b = ln_plan(rows, int(width), type, false);
-  return a.grid > b.grid ? a.grid : b.grid;
+  int most = 0;
+  for (int kept : {1, type == kTypeFp32 ? 4 : 2})
+    for (bool aligned : {false, true}) {
+      const LnPlan p = ln_plan(rows, int(width), type, aligned, kept);
+      if (p.grid > most) most = p.grid;
+    }
+  return most;
 }
 
 int mek_layer_norm_fwd(const void* x, int type, const void* weight, const void* bias, int param_type, void* y,
@@ -449,7 +691,7 @@ int mek_layer_norm_fwd(const void* x, int type, const void* weight, const void* 
   if (codes && width > 200704)
     return fail(MEK_ERR_UNSUPPORTED, "layer_norm_fwd: the 8-bit checkpoint holds rows of up to 200,704 columns");
   const LnPlan p = ln_plan(rows, int(width), type, ln_aligned(type, width, x_row_stride, x, y, nullptr) &&
-                                                       reinterpret_cast<uintptr_t>(codes) % 8 == 0);
+                                                       reinterpret_cast<uintptr_t>(codes) % 8 == 0, 0);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
 #define MEK_LN_FWD(T, VEC, G, NV) \
   ln_fwd<T, VEC, G, NV>(p, x, x_row_stride, weight, bias, param_type, y, mean, rstd, codes, rows, int(width), eps, s)
@@ -479,7 +721,8 @@ int mek_layer_norm_bwd(const void* dy, const void* x, int type, const uint8_t* c
   if (int rc = check_ln("layer_norm_bwd", type, param_type, rows, width, codes ? 0 : x_row_stride)) return rc;
   const LnPlan p =
       ln_plan(rows, int(width), type, ln_aligned(type, width, codes ? 0 : x_row_stride, dy, dx, codes ? nullptr : x) &&
-                                          reinterpret_cast<uintptr_t>(codes) % 8 == 0);
+                                          reinterpret_cast<uintptr_t>(codes) % 16 == 0,
+              codes ? 1 : type == kTypeFp32 ? 4 : 2);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int w = int(width);
   auto main_launch = [&]() -> int {

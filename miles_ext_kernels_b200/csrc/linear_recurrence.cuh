@@ -39,41 +39,6 @@ constexpr int kGlrTile = kGlrTokens * kGlrWarps;     // tokens a block owns
 constexpr int kGlrChannels = 64;                     // channels a block owns
 constexpr float kGlrReset = -1.0f;                   // A of a run that holds a sequence's first token
 
-// Two FP32 numbers in one register pair: the packed operations halve the instructions of a lane's two channels.
-typedef unsigned long long Two;
-__device__ __forceinline__ Two two(float x, float y) {
-  Two v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-  return v;
-}
-__device__ __forceinline__ Two two(float x) { return two(x, x); }
-__device__ __forceinline__ float2 split(Two v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-  Two d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ Two mul2(Two a, Two b) {
-  Two d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ Two add2(Two a, Two b) {
-  Two d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
-__device__ __forceinline__ Two sub2(Two a, Two b) {
-  Two d;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 __device__ __forceinline__ float clamped(float g) {  // NaN stays
   float v;
   asm("max.NaN.f32 %0, %1, 0fC2B00000;" : "=f"(v) : "f"(g));   // -88
@@ -161,15 +126,6 @@ __device__ __forceinline__ Span span_of(const Sequences& s, int t0) {
     if (__ballot_sync(0xffffffffu, in) != 0xffffffffu) break;
   }
   return span;
-}
-
-template <typename T>
-__device__ __forceinline__ Two widened(const Vec<T, 2>& v) { return two(to_float(v.e[0]), to_float(v.e[1])); }
-template <typename T>
-__device__ __forceinline__ Vec<T, 2> narrowed(Two v) {
-  const float2 f = split(v);
-  const float a[2] = {f.x, f.y};
-  return pack<T, 2>(a);
 }
 
 // One tensor [batch, tokens, channels] of a call: its map (kTma) or its base and strides (elements).

@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   const Edges edges(s.seq, span_of(s.seq, t0), at.b, t0);
   const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
   const Two d1 = edges.end >= 0 ? load_state<kTma>(p.d_final, s, at, edges.end_seq) : two(0.f);
-  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
+  if constexpr (kTma) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
   {
     Two A, B, D;
     if (edges.kind == kInside) walk_tokens<X, G, true, false>(decay, xs, ds, edges, s0, d1, A, B, D);

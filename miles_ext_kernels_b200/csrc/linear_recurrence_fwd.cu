@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   }
   const Edges edges(s.seq, span_of(s.seq, t0), at.b, t0);
   const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
-  if constexpr (kTma) arrived = mbar_wait(&sh.arrived[warp], 0);
+  if constexpr (kTma) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
   Two A, B, none;
   if (edges.kind == kInside) walk_tokens<X, G, false, false>(decay, xs, xs, edges, none, none, A, B, none);
   else walk_tokens<X, G, false, true>(decay, xs, xs, edges, s0, none, A, B, none);

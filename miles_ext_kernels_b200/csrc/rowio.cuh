@@ -7,6 +7,8 @@
 #include <cuda_fp8.h>
 #include <stdint.h>
 
+#include "umma.cuh"
+
 namespace mek {
 
 enum : int { kTypeBf16 = 0, kTypeFp16 = 1, kTypeFp32 = 2 };
@@ -40,6 +42,50 @@ __device__ __forceinline__ Vec<T, N> pack(const float (&v)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) raw.e[i] = from_float<T>(v[i]);
   return raw;
+}
+
+// Two FP32 numbers in one register pair: the packed operations halve the instructions of a lane's two channels.
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float x, float y) {
+  Two v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+__device__ __forceinline__ Two two(float x) { return two(x, x); }
+__device__ __forceinline__ float2 split(Two v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+__device__ __forceinline__ Two sub2(Two a, Two b) {
+  Two d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ Two widened(const Vec<T, 2>& v) { return two(to_float(v.e[0]), to_float(v.e[1])); }
+template <typename T>
+__device__ __forceinline__ Vec<T, 2> narrowed(Two v) {
+  const float2 f = split(v);
+  const float a[2] = {f.x, f.y};
+  return pack<T, 2>(a);
 }
 
 // Element i of a parameter vector in one of the three types (a launch-uniform switch).
@@ -82,6 +128,14 @@ __device__ __forceinline__ void from_e4m3(const Vec<uint8_t, N>& codes, float (&
       v[i] = f.x, v[i + 1] = f.y;
     }
   }
+}
+
+// mbar_wait for copies that are on their way as a rule: the first looks go without the timer, whose reading costs more than
+// a look (and is shared by the SM).
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
+  for (int looks = 0; looks < 256; ++looks)
+    if (mbar_try_wait(bar, parity)) return true;
+  return mbar_wait(bar, parity);
 }
 
 __device__ __forceinline__ float warp_sum(float x) {
