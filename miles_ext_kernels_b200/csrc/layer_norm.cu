@@ -161,8 +161,12 @@ __device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t b
 }
 template <int VEC, int G>
 constexpr bool kLnStreams = VEC > 1 && G >= 128;
+// Blocks an SM: about 80 registers a thread for the forward, 128 for the backward, whose sums take a third of them (a group
+// of 1,024 has 64 either way).
 template <int G>
-constexpr int kLnBlocks = G <= 128 ? 6 : G == 256 ? 3 : 1;  // blocks an SM, for about 80 registers a thread (1,024: 64)
+constexpr int kLnFwdBlocks = G <= 128 ? 6 : G == 256 ? 3 : 1;
+template <int G>
+constexpr int kLnBwdBlocks = G <= 128 ? 4 : G == 256 ? 2 : 1;
 // Groups of 1,024 threads have 64 registers: their parameters stay in shared memory.
 template <int G>
 constexpr bool kLnParamsShared = G == 1024;
@@ -201,7 +205,7 @@ struct RowParams {
 
 // x [rows, width] with a row stride; y and codes dense.  Block b takes rows (or groups of rows) b, b + gridDim.x, ...
 template <typename T, int VEC, int G, int NV>
-__global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G>) layer_norm_fwd_kernel(
+__global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlocks<G>) layer_norm_fwd_kernel(
     const T* __restrict__ x, int64_t x_stride, const void* __restrict__ weight, const void* __restrict__ bias,
     int param_type, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
     uint8_t* __restrict__ codes, int64_t rows, int width, float eps, int slots) {
@@ -311,10 +315,9 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G
 }
 
 // kCodes: unit comes from the 8-bit checkpoint, x and mean are not read.  partial [gridDim.x, 2, width] (or NULL).
-// A streamed row is read from shared memory twice, for the sums and for dx (its slot is filled again once the block has
-// passed the next row's barrier); a row in registers stays there.
+// A row stays in registers, as it came, between the sums and dx.
 template <typename T, int VEC, int G, int NV, bool kCodes, bool kStream>
-__global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G>) layer_norm_bwd_kernel(
+__global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlocks<G>) layer_norm_bwd_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ codes,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const void* __restrict__ weight,
     int param_type, T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width, int slots) {
@@ -360,18 +363,17 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G
   };
   ahead(first);
   __syncthreads();
-  int slot = 0, parity = 0, phase = 0, before = -1;
+  int slot = 0, parity = 0, phase = 0;
   for (int64_t r = first; r < rows; r += step, phase ^= 1) {
     const float rstd = next_rstd;
     const Two mean = two(next_mean), scale = two(rstd);
     bool arrived = true;
     RowPart<T, VEC, G, NV> g_part;
     RowPart<Kept, VEC, G, NV> k_part;
-    const T* g_row = reinterpret_cast<const T*>(smem + slot * bytes);
-    const Kept* k_row = reinterpret_cast<const Kept*>(smem + slot * bytes + dy_bytes);
     if constexpr (kStream) {
       arrived = mbar_wait_soon(&s_full[slot], parity);
-      g_part.load(g_row, lane, width), k_part.load(k_row, lane, width);
+      g_part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
+      k_part.load(reinterpret_cast<const Kept*>(smem + slot * bytes + dy_bytes), lane, width);
     } else {
       g_part = g_next, k_part = k_next;
     }
@@ -392,15 +394,11 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBlocks<G
     }
     const float2 a = split(s1), c = split(s2);
     const float2 sums = group_sum<G>(arrived ? a.x + a.y : __int_as_float(0x7fffffff), c.x + c.y, s_part, phase);
-    if constexpr (kStream) {
-      if (threadIdx.x == 0 && before >= 0 && r + (slots - 1) * step < rows) fill(before, r + (slots - 1) * step);
-      g_part.load(g_row, lane, width), k_part.load(k_row, lane, width);
-    }
+    if (kStream && threadIdx.x == 0 && r + slots * step < rows) fill(slot, r + slots * step);  // all have read the row
     const Two m1 = two(sums.x * inv_width), m2 = two(-(sums.y * inv_width));
     store_row<T, VEC, G, NV>(dx + r * width, lane, width, [&](int q) {
       return mul2(fma2(unit(q), m2, sub2(mul2(g_part.pair(q), w.pair(q, lane)), m1)), scale);
     });
-    before = slot;
     if (kStream && ++slot == slots) slot = 0, parity ^= 1;
   }
   if (partial == nullptr) return;
@@ -575,7 +573,8 @@ LnPlan ln_plan(int64_t rows, int width, int type, bool aligned, int kept_size) {
     while (g * p.vec * p.nv < width) p.nv *= 2;
     break;
   }
-  int blocks = p.group == 0 ? 2 : p.group <= 128 ? kLnBlocks<128> : p.group == 256 ? kLnBlocks<256> : kLnBlocks<512>;
+  int blocks = p.group == 0 || p.group == 256 ? 2 : p.group <= 128 ? kLnBwdBlocks<128> : 1;
+  if (kept_size == 0 && p.group > 0) blocks = p.group <= 128 ? kLnFwdBlocks<128> : p.group == 256 ? kLnFwdBlocks<256> : 1;
   if (p.vec > 1 && p.group >= 128 && (kept_size != 1 || width % 16 == 0)) {  // bulk copies move multiples of 16 bytes
     const int64_t bytes = int64_t(width) * (size + kept_size), params = p.group == 1024 ? width * (kept_size ? 4 : 8) : 0;
     const int64_t fit = ((p.group == 1024 ? 210 << 10 : 160 << 10) - params) / (blocks * bytes);
