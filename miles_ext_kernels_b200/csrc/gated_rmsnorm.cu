@@ -26,8 +26,19 @@ constexpr int kNormMaxBlocks = 148 * 4;
 struct RowView {
   const __nv_bfloat16* base;
   int64_t token_stride, head_stride;
-  __device__ __forceinline__ const __nv_bfloat16* row(int64_t r, int heads) const {
-    return base + (r / heads) * token_stride + (r % heads) * head_stride;
+  __device__ __forceinline__ const __nv_bfloat16* row(int64_t token, int64_t head) const {
+    return base + token * token_stride + head * head_stride;
+  }
+};
+// Rows r0 and r0 + 1 (the last row for what lies past it) as (token, head): one division for both.
+struct TwoRows {
+  int64_t token[2], head[2];
+  __device__ __forceinline__ TwoRows(int64_t r0, int64_t rows, int heads) {
+    const int64_t r = r0 < rows ? r0 : rows - 1;
+    token[0] = r / heads, head[0] = r - token[0] * heads;
+    const bool turn = head[0] + 1 == heads, more = r0 + 1 < rows;
+    token[1] = token[0] + (more && turn ? 1 : 0);
+    head[1] = !more ? head[0] : turn ? 0 : head[0] + 1;
   }
 };
 
@@ -75,11 +86,11 @@ __global__ void __launch_bounds__(256) gated_rmsnorm_fwd_kernel(RowView x, RowVi
   const int64_t r0 = int64_t(blockIdx.x) * kNormRowsPerBlock + half * 2;
   float wv[8], xv[2][8], zv[2][8];
   load8(w, l16, wv);
+  const TwoRows at(r0, rows, heads);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {  // both rows' loads in flight before any arithmetic
-    const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
-    load8(x.row(r, heads), l16, xv[i]);
-    load8(z.row(r, heads), l16, zv[i]);
+    load8(x.row(at.token[i], at.head[i]), l16, xv[i]);
+    load8(z.row(at.token[i], at.head[i]), l16, zv[i]);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -103,57 +114,76 @@ __global__ void __launch_bounds__(256) gated_rmsnorm_fwd_kernel(RowView x, RowVi
       }
       if (r0 + i < rows) {
         const int64_t r = r0 + i;
-        reinterpret_cast<Vec<uint8_t, 8>*>(keep.n_codes + r * 128)[l16] = to_e4m3(n);
-        reinterpret_cast<Vec<uint8_t, 8>*>(keep.z_codes + r * 128)[l16] = to_e4m3(scaled);
+        store_codes(keep.n_codes + r * 128 + l16 * 8, n);
+        store_codes(keep.z_codes + r * 128 + l16 * 8, scaled);
         if (l16 == 0) keep.z_exponent[r] = uint8_t(e + 127), keep.rstd[r] = rstd;
       }
     }
   }
 }
 
-// The backward from the checkpoint; formulas as below with n and z as the codes hold them.
-__global__ void __launch_bounds__(256) gated_rmsnorm_bwd_kept_kernel(const __nv_bfloat16* __restrict__ dy,
-                                                                     NormCheckpoint kept,
-                                                                     const __nv_bfloat16* __restrict__ w,
-                                                                     __nv_bfloat16* __restrict__ dx,
-                                                                     __nv_bfloat16* __restrict__ dz,
-                                                                     float* __restrict__ dw_partial, int64_t rows) {
+// The backward from the checkpoint; formulas as below with n and z as the codes hold them.  A half-warp's row of the next
+// group is loaded, as it lies in memory, as soon as the present one is decoded.
+struct KeptRow {
+  Codes<8> n, z;
+  uint4 dy;
+  float rstd;
+  uint8_t exponent;
+  __device__ __forceinline__ void load(const NormCheckpoint& kept, const __nv_bfloat16* dy_in, int64_t r, int l16) {
+    n = load_codes<8>(kept.n_codes + r * 128 + l16 * 8);
+    z = load_codes<8>(kept.z_codes + r * 128 + l16 * 8);
+    dy = __ldg(reinterpret_cast<const uint4*>(dy_in + r * 128) + l16);
+    rstd = kept.rstd[r];
+    exponent = kept.z_exponent[r];
+  }
+};
+__global__ void __launch_bounds__(256, 3) gated_rmsnorm_bwd_kept_kernel(const __nv_bfloat16* __restrict__ dy,
+                                                                        NormCheckpoint kept,
+                                                                        const __nv_bfloat16* __restrict__ w,
+                                                                        __nv_bfloat16* __restrict__ dx,
+                                                                        __nv_bfloat16* __restrict__ dz,
+                                                                        float* __restrict__ dw_partial, int64_t rows) {
   __shared__ float s_dw[16][128];
   const int l16 = threadIdx.x & 15, half = threadIdx.x >> 4;
   float wv[8], acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   load8(w, l16, wv);
-  for (int64_t group = blockIdx.x; group * kNormRowsPerBlock < rows; group += gridDim.x) {
-    const int64_t r0 = group * kNormRowsPerBlock + half * 2;
-    float n[2][8], zv[2][8], gv[2][8], rstd[2], up[2];
+  const int64_t step = int64_t(gridDim.x) * kNormRowsPerBlock, first = int64_t(blockIdx.x) * kNormRowsPerBlock;
+  KeptRow row[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) row[i].load(kept, dy, min(first + half * 2 + i, rows - 1), l16);
+  for (int64_t group = first; group < rows; group += step) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
-      from_e4m3(reinterpret_cast<const Vec<uint8_t, 8>*>(kept.n_codes + r * 128)[l16], n[i]);
-      from_e4m3(reinterpret_cast<const Vec<uint8_t, 8>*>(kept.z_codes + r * 128)[l16], zv[i]);
-      load8(dy + r * 128, l16, gv[i]);
-      rstd[i] = kept.rstd[r];
-      up[i] = power_of_two(int(kept.z_exponent[r]) - 127);
-    }
+      const int64_t r = group + half * 2 + i;
+      const bool live = r < rows;  // uniform over the half-warp
+      const float up = power_of_two(int(row[i].exponent) - 127), rstd = row[i].rstd;
+      float n[8], zv[8], gv[8], dn[8], dzv[8], dxv[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const bool live = r0 + i < rows;  // uniform over the half-warp
-      float dot = 0.f, dn[8], dzv[8], dxv[8];
+      for (int q = 0; q < 4; ++q) {
+        const float2 a = code_pair(row[i].n, q), b = code_pair(row[i].z, q);
+        n[2 * q] = a.x, n[2 * q + 1] = a.y, zv[2 * q] = b.x, zv[2 * q + 1] = b.y;
+      }
+      const float2 g0 = unpack_bf16(row[i].dy.x), g1 = unpack_bf16(row[i].dy.y), g2 = unpack_bf16(row[i].dy.z),
+                   g3 = unpack_bf16(row[i].dy.w);
+      gv[0] = g0.x, gv[1] = g0.y, gv[2] = g1.x, gv[3] = g1.y, gv[4] = g2.x, gv[5] = g2.y, gv[6] = g3.x, gv[7] = g3.y;
+      if (r + step < rows) row[i].load(kept, dy, r + step, l16);
+      float dot = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float z = zv[i][j] * up[i];
+        const float z = zv[j] * up;
         const float s = __fdividef(1.0f, 1.0f + __expf(-z));
-        const float a = gv[i][j] * (z * s);
+        const float a = gv[j] * (z * s);
         dn[j] = a * wv[j];
-        dot = fmaf(dn[j], n[i][j], dot);
-        dzv[j] = gv[i][j] * n[i][j] * wv[j] * s * (1.0f + z * (1.0f - s));
-        if (live) acc[j] = fmaf(a, n[i][j], acc[j]);
+        dot = fmaf(dn[j], n[j], dot);
+        dzv[j] = gv[j] * n[j] * wv[j] * s * (1.0f + z * (1.0f - s));
+        if (live) acc[j] = fmaf(a, n[j], acc[j]);
       }
       const float mean = half_warp_sum(dot) * (1.0f / 128.0f);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dxv[j] = rstd[i] * (dn[j] - n[i][j] * mean);
+      for (int j = 0; j < 8; ++j) dxv[j] = rstd * (dn[j] - n[j] * mean);
       if (live) {
-        store8(dx + (r0 + i) * 128, l16, dxv);
-        store8(dz + (r0 + i) * 128, l16, dzv);
+        store8(dx + r * 128, l16, dxv);
+        store8(dz + r * 128, l16, dzv);
       }
     }
   }
@@ -184,11 +214,12 @@ __global__ void __launch_bounds__(256) gated_rmsnorm_bwd_kernel(const __nv_bfloa
   for (int64_t group = blockIdx.x; group * kNormRowsPerBlock < rows; group += gridDim.x) {
     const int64_t r0 = group * kNormRowsPerBlock + half * 2;
     float xv[2][8], zv[2][8], gv[2][8];
+    const TwoRows at(r0, rows, heads);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int64_t r = r0 + i < rows ? r0 + i : rows - 1;
-      load8(x.row(r, heads), l16, xv[i]);
-      load8(z.row(r, heads), l16, zv[i]);
+      load8(x.row(at.token[i], at.head[i]), l16, xv[i]);
+      load8(z.row(at.token[i], at.head[i]), l16, zv[i]);
       load8(dy + r * 128, l16, gv[i]);
     }
 #pragma unroll

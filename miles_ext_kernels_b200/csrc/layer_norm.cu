@@ -29,7 +29,8 @@ constexpr int kLnMaxSlots = 8;
 // neighbouring columns of one access, or (VEC = 1, NV even) the columns of two accesses.
 template <typename T, int VEC, int G, int NV>
 struct RowShape {
-  static constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, kWarps = G / 32, kPairs = NV * VEC / 2;
+  static constexpr int kThreads = G < 128 ? 128 : G, kRows = kThreads / G, kWarps = G < 32 ? 1 : G / 32;
+  static constexpr int kPairs = NV * VEC / 2, kSide = G < 32 ? 32 / G : 1;  // rows a warp holds side by side
   static_assert(NV * VEC % 2 == 0, "pairs");
   static __device__ __forceinline__ int column(int lane, int q, int i) {
     if constexpr (VEC == 1) return (2 * q + i) * G + lane;
@@ -39,7 +40,7 @@ struct RowShape {
   static __device__ __forceinline__ int count(int w, int width) {
     int n = 0;
 #pragma unroll
-    for (int v = 0; v < NV; ++v) n += min(max(width - (v * G + w * 32) * VEC, 0), 32 * VEC);
+    for (int v = 0; v < NV; ++v) n += min(max(width - (v * G + w * 32) * VEC, 0), min(G, 32) * VEC);
     return n;
   }
 };
@@ -67,24 +68,22 @@ struct RowPart {
 };
 template <int VEC, int G, int NV>
 struct RowPart<uint8_t, VEC, G, NV> {
-  Vec<uint8_t, VEC> raw[NV];
+  Codes<VEC> raw[NV];
   __device__ __forceinline__ void load(const uint8_t* row, int lane, int width) {
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int c = (v * G + lane) * VEC;
-      if (c < width) raw[v] = *reinterpret_cast<const Vec<uint8_t, VEC>*>(row + c);
-      else
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) raw[v].e[i] = 0;
+      if (c < width) raw[v] = load_codes<VEC>(row + c);
+      else raw[v].clear();
     }
   }
   __device__ __forceinline__ Two pair(int q) const {
-    Vec<uint8_t, 2> codes;
-    if constexpr (VEC == 1) codes = {{raw[2 * q].e[0], raw[2 * q + 1].e[0]}};
-    else codes = {{raw[q / (VEC / 2)].e[q % (VEC / 2) * 2], raw[q / (VEC / 2)].e[q % (VEC / 2) * 2 + 1]}};
-    float f[2];
-    from_e4m3(codes, f);
-    return two(f[0], f[1]);
+    if constexpr (VEC == 1) {
+      return two(code_value(raw[2 * q].byte), code_value(raw[2 * q + 1].byte));
+    } else {
+      const float2 f = code_pair(raw[q / (VEC / 2)], q % (VEC / 2));
+      return two(f.x, f.y);
+    }
   }
 };
 template <typename E, int VEC, int G, int NV, typename Value>  // value(q) -> Two
@@ -110,7 +109,7 @@ __device__ __forceinline__ void store_row(E* row, int lane, int width, Value val
   }
 }
 template <int VEC, int G, int NV, typename Value>
-__device__ __forceinline__ void store_codes(uint8_t* row, int lane, int width, Value value) {
+__device__ __forceinline__ void store_row_codes(uint8_t* row, int lane, int width, Value value) {
 #pragma unroll
   for (int v = 0; v < NV; ++v) {
     const int c = (v * G + lane) * VEC;
@@ -118,8 +117,8 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int lane, int width, V
       if (v % 2) continue;
       const float2 f = split(value(v / 2));
       const float a[1] = {f.x}, b[1] = {f.y};
-      if (c < width) row[c] = to_e4m3(a).e[0];
-      if (c + G < width) row[c + G] = to_e4m3(b).e[0];
+      if (c < width) store_codes(row + c, a);
+      if (c + G < width) store_codes(row + c + G, b);
     } else {
       if (c >= width) continue;
       float f[VEC];
@@ -128,16 +127,24 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int lane, int width, V
         const float2 p = split(value(v * (VEC / 2) + i));
         f[2 * i] = p.x, f[2 * i + 1] = p.y;
       }
-      *reinterpret_cast<Vec<uint8_t, VEC>*>(row + c) = to_e4m3(f);
+      store_codes(row + c, f);
     }
   }
+}
+
+// Over the lanes of a group inside a warp.
+template <int G>
+__device__ __forceinline__ float lane_sum(float x) {
+#pragma unroll
+  for (int m = min(G, 32) / 2; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+  return x;
 }
 
 // Sums over a group of two values, the warps' sums through shared memory (`phase` alternates: one barrier a row).
 template <int G>
 __device__ __forceinline__ float2 group_sum(float a, float b, float2 (*part)[32], int phase) {
-  a = warp_sum(a), b = warp_sum(b);
-  if constexpr (G == 32) return make_float2(a, b);
+  a = lane_sum<G>(a), b = lane_sum<G>(b);
+  if constexpr (G <= 32) return make_float2(a, b);
   if (threadIdx.x % 32 == 0) part[phase][threadIdx.x / 32] = make_float2(a, b);
   __syncthreads();
   if constexpr (G <= 256) {
@@ -161,26 +168,32 @@ __device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t b
 }
 template <int VEC, int G>
 constexpr bool kLnStreams = VEC > 1 && G >= 128;
+// Rows ahead in registers: where a warp holds rows of its own, four of up to 16 bytes a thread or two of more (narrow rows
+// would keep few bytes in flight otherwise), else one.
+template <typename T, int VEC, int G, int NV>
+constexpr int kLnDepth = G >= 128 ? 1 : NV * VEC * int(sizeof(T)) <= 16 ? 4 : 2;
 // Blocks an SM: about 80 registers a thread for the forward, 128 for the backward, whose sums take a third of them (a group
 // of 1,024 has 64 either way).
 template <int G>
-constexpr int kLnFwdBlocks = G <= 128 ? 6 : G == 256 ? 3 : 1;
+constexpr int kLnFwdBlocks = G <= 32 ? 5 : G == 128 ? 6 : G == 256 ? 3 : 1;
 template <int G>
 constexpr int kLnBwdBlocks = G <= 128 ? 4 : G == 256 ? 2 : 1;
-// Groups of 1,024 threads have 64 registers: their parameters stay in shared memory.
-template <int G>
-constexpr bool kLnParamsShared = G == 1024;
+// The widest rows leave no registers for the parameters, which stay in shared memory: 32 elements a thread of 128 registers
+// (16-bit rows; with 1,024 threads of 64 registers the backward spilled and took 343 us for 8,192 x 16,384 instead of
+// 316), or 1,024 threads.
+template <int VEC, int G, int NV>
+constexpr bool kLnParamsShared = G == 1024 || NV * VEC == 32;
 
 // The parameters of a thread's columns, FP32.
 template <typename T, int VEC, int G, int NV>
 struct RowParams {
   typedef RowShape<T, VEC, G, NV> Shape;
-  Two kept[kLnParamsShared<G> ? 1 : Shape::kPairs];
+  Two kept[kLnParamsShared<VEC, G, NV> ? 1 : Shape::kPairs];
   const float* shared;
   int last;  // columns past the row's end read its last parameters, and nobody what comes of it
   __device__ __forceinline__ void load(const void* p, int type, float missing, float* room, int lane, int width) {
     shared = room, last = VEC == 1 ? width - 1 : width - 2;
-    if constexpr (kLnParamsShared<G>) {
+    if constexpr (kLnParamsShared<VEC, G, NV>) {
       for (int c = lane; c < width; c += G) room[c] = p ? load_param(p, type, c) : missing;
     } else {
 #pragma unroll
@@ -196,7 +209,7 @@ struct RowParams {
     }
   }
   __device__ __forceinline__ Two pair(int q, int lane) const {
-    if constexpr (!kLnParamsShared<G>) return kept[q];
+    if constexpr (!kLnParamsShared<VEC, G, NV>) return kept[q];
     else if constexpr (VEC == 1)
       return two(shared[min(Shape::column(lane, q, 0), last)], shared[min(Shape::column(lane, q, 1), last)]);
     else return *reinterpret_cast<const Two*>(shared + min(Shape::column(lane, q, 0), last));
@@ -235,11 +248,19 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
   const int count = Shape::count(warp, width);
   const float inv_count = count ? 1.f / float(count) : 0.f, inv_width = 1.f / float(width);
   const bool full = Shape::column(lane, kPairs - 1, 1) < width;  // no column past the row's end
-  RowPart<T, VEC, G, NV> part;
-  if (!kStream && first < rows) part.load(x + first * x_stride, lane, width);
+  constexpr int kDepth = kStream ? 1 : kLnDepth<T, VEC, G, NV>;
+  RowPart<T, VEC, G, NV> parts[kDepth];
+  if constexpr (!kStream) {
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k) {
+      if (Shape::kSide > 1) parts[k].load(x, lane, 0);  // zeros where a warp's last rows are not all there
+      if (first + k * step < rows) parts[k].load(x + (first + k * step) * x_stride, lane, width);
+    }
+  }
   __syncthreads();
   int slot = 0, parity = 0, phase = 0;
-  for (int64_t r = first; r < rows; r += step, phase ^= 1) {
+  auto one_row = [&](int64_t r, RowPart<T, VEC, G, NV>& part) {
+    const bool live = Shape::kSide == 1 || r < rows;  // rows side by side in a warp go through its shuffles together
     bool arrived = true;
     if constexpr (kStream) {
       arrived = mbar_wait_soon(&s_full[slot], parity);
@@ -249,12 +270,12 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
 #pragma unroll
     for (int q = 0; q < kPairs; ++q) xv[q] = part.pair(q), sum = add2(sum, xv[q]);
     if constexpr (!kStream)
-      if (r + step < rows) part.load(x + (r + step) * x_stride, lane, width);
+      if (r + kDepth * step < rows) part.load(x + (r + kDepth * step) * x_stride, lane, width);
     // this warp's mean and squares about it; a mean is rounded before it is subtracted, whether or not it is stored: the
     // same y either way
     float2 s = split(sum);
     if (!arrived) s.x = __int_as_float(0x7fffffff);
-    float total = warp_sum(s.x + s.y);
+    float total = lane_sum<G>(s.x + s.y);
     float mean = __fmul_rn(total, inv_count);
     Two squares = two(0.f);
     const Two mean2 = two(mean);
@@ -273,7 +294,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
       }
     }
     s = split(squares);
-    float m2 = warp_sum(s.x + s.y);
+    float m2 = lane_sum<G>(s.x + s.y);
     if constexpr (G > 32) {  // the warps' by Chan's rule
       if (threadIdx.x % 32 == 0) s_part[phase][warp] = make_float2(mean, m2);
       __syncthreads();
@@ -301,16 +322,25 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
       }
     }
     const float rstd = rsqrtf(m2 * inv_width + eps);
-    if (lane == 0) {
+    if (lane == 0 && live) {
       if (mean_out) mean_out[r] = mean;
       if (rstd_out) rstd_out[r] = rstd;
     }
     const Two m = two(mean), scale = two(rstd);
 #pragma unroll
     for (int q = 0; q < kPairs; ++q) xv[q] = mul2(sub2(xv[q], m), scale);  // unit
-    store_row<T, VEC, G, NV>(y + r * width, lane, width, [&](int q) { return fma2(xv[q], w.pair(q, lane), b.pair(q, lane)); });
-    if (codes) store_codes<VEC, G, NV>(codes + r * width, lane, width, [&](int q) { return xv[q]; });
+    if (live) {
+      store_row<T, VEC, G, NV>(y + r * width, lane, width, [&](int q) { return fma2(xv[q], w.pair(q, lane), b.pair(q, lane)); });
+      if (codes) store_row_codes<VEC, G, NV>(codes + r * width, lane, width, [&](int q) { return xv[q]; });
+    }
     if (kStream && ++slot == slots) slot = 0, parity ^= 1;
+    phase ^= 1;
+  };
+  const int side = Shape::kSide == 1 ? 0 : int(threadIdx.x % 32) / G;
+  for (int64_t r = first; r - side < rows; r += kDepth * step) {
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k)
+      if (r - side + k * step < rows) one_row(r + k * step, parts[k]);
   }
 }
 
@@ -352,21 +382,28 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
 #pragma unroll
   for (int q = 0; q < kPairs; ++q) dw[q] = db[q] = two(0.f);
   const float inv_width = 1.f / float(width);
-  float next_rstd = 0.f, next_mean = 0.f;  // the statistics are a row ahead
-  RowPart<T, VEC, G, NV> g_next;
-  RowPart<Kept, VEC, G, NV> k_next;
-  auto ahead = [&](int64_t r) {
+  constexpr int kDepth = kStream || G >= 128 ? 1 : kLnDepth<T, VEC, G, NV> / 2;
+  float ahead_rstd[kDepth], ahead_mean[kDepth];  // the statistics are ahead as well
+  RowPart<T, VEC, G, NV> g_parts[kDepth];
+  RowPart<Kept, VEC, G, NV> k_parts[kDepth];
+  auto ahead = [&](int64_t r, int k) {
     if (r >= rows) return;
-    next_rstd = rstd_in[r];
-    if constexpr (!kCodes) next_mean = mean_in[r];
-    if constexpr (!kStream) g_next.load(dy + r * width, lane, width), k_next.load(kept_row(r), lane, width);
+    ahead_rstd[k] = rstd_in[r];
+    if constexpr (!kCodes) ahead_mean[k] = mean_in[r];
+    if constexpr (!kStream) g_parts[k].load(dy + r * width, lane, width), k_parts[k].load(kept_row(r), lane, width);
   };
-  ahead(first);
+#pragma unroll
+  for (int k = 0; k < kDepth; ++k) {
+    ahead_rstd[k] = ahead_mean[k] = 0.f;
+    if constexpr (Shape::kSide > 1) g_parts[k].load(dy, lane, 0), k_parts[k].load(kept_row(0), lane, 0);
+    ahead(first + k * step, k);
+  }
   __syncthreads();
   int slot = 0, parity = 0, phase = 0;
-  for (int64_t r = first; r < rows; r += step, phase ^= 1) {
-    const float rstd = next_rstd;
-    const Two mean = two(next_mean), scale = two(rstd);
+  auto one_row = [&](int64_t r, int k) {
+    const bool live = Shape::kSide == 1 || r < rows;
+    const float rstd = ahead_rstd[k];
+    const Two mean = two(ahead_mean[k]), scale = two(rstd);
     bool arrived = true;
     RowPart<T, VEC, G, NV> g_part;
     RowPart<Kept, VEC, G, NV> k_part;
@@ -375,9 +412,10 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
       g_part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
       k_part.load(reinterpret_cast<const Kept*>(smem + slot * bytes + dy_bytes), lane, width);
     } else {
-      g_part = g_next, k_part = k_next;
+      g_part = g_parts[k], k_part = k_parts[k];
     }
-    ahead(r + step);
+    ahead(r + kDepth * step, k);
+    if (Shape::kSide > 1 && !live) g_part.load(dy, lane, 0), k_part.load(kept_row(0), lane, 0);  // zeros add nothing
     auto unit = [&](int q) {
       const Two v = k_part.pair(q);
       if constexpr (kCodes) return v;
@@ -396,10 +434,17 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
     const float2 sums = group_sum<G>(arrived ? a.x + a.y : __int_as_float(0x7fffffff), c.x + c.y, s_part, phase);
     if (kStream && threadIdx.x == 0 && r + slots * step < rows) fill(slot, r + slots * step);  // all have read the row
     const Two m1 = two(sums.x * inv_width), m2 = two(-(sums.y * inv_width));
-    store_row<T, VEC, G, NV>(dx + r * width, lane, width, [&](int q) {
+    if (live) store_row<T, VEC, G, NV>(dx + r * width, lane, width, [&](int q) {
       return mul2(fma2(unit(q), m2, sub2(mul2(g_part.pair(q), w.pair(q, lane)), m1)), scale);
     });
     if (kStream && ++slot == slots) slot = 0, parity ^= 1;
+    phase ^= 1;
+  };
+  const int side = Shape::kSide == 1 ? 0 : int(threadIdx.x % 32) / G;
+  for (int64_t r = first; r - side < rows; r += kDepth * step) {
+#pragma unroll
+    for (int k = 0; k < kDepth; ++k)
+      if (r - side + k * step < rows) one_row(r + k * step, k);
   }
   if (partial == nullptr) return;
   float* mine = partial + int64_t(blockIdx.x) * 2 * width;
@@ -491,17 +536,14 @@ __global__ void __launch_bounds__(kWideThreads) layer_norm_wide_fwd_kernel(
       const float unit[1] = {(to_float(row[c]) - mean) * rstd};
       const float w = weight ? load_param(weight, param_type, c) : 1.f, b = bias ? load_param(bias, param_type, c) : 0.f;
       y[r * width + c] = from_float<T>(fmaf(unit[0], w, b));
-      if (codes) codes[r * width + c] = to_e4m3(unit).e[0];
+      if (codes) store_codes(codes + r * width + c, unit);
     }
   }
 }
 template <typename T>
 __device__ __forceinline__ float wide_unit(const T* x_row, const uint8_t* code_row, int c, float mean, float rstd) {
   if (code_row == nullptr) return (to_float(x_row[c]) - mean) * rstd;
-  Vec<uint8_t, 1> code{{code_row[c]}};
-  float unit[1];
-  from_e4m3(code, unit);
-  return unit[0];
+  return code_value(code_row[c]);
 }
 template <typename T>
 __global__ void __launch_bounds__(kWideThreads) layer_norm_wide_dx_kernel(
@@ -559,14 +601,14 @@ struct LnPlan {
 
 // vec: elements per access, 16 bytes where every row starts on a 16-byte boundary, else one.  The smallest group
 // of threads that holds a row in at most 16 elements a thread where accesses are wide, 8 (at last 16) where they are
-// not.  A row of wide accesses that takes a whole block is streamed (kept_size: bytes an element of what the backward
+// not (8 elements in a part of a warp).  A row of wide accesses that takes a whole block is streamed (kept_size: bytes an element of what the backward
 // reads besides dy, 0 for the forward): as many rows in flight as 160 KB an SM hold, two to eight.
 LnPlan ln_plan(int64_t rows, int width, int type, bool aligned, int kept_size) {
   const int size = type == kTypeFp32 ? 4 : 2;
   LnPlan p{aligned ? 16 / size : 1, 0, 0, 0, 0};
-  static const int groups[] = {32, 128, 256, 512, 1024};
+  static const int groups[] = {8, 16, 32, 128, 256, 512, 1024};
   for (int g : groups) {
-    const int most = p.vec > 1 ? 16 / p.vec : g == 1024 ? 16 : 8;
+    const int most = p.vec == 1 ? (g == 1024 ? 16 : 8) : (g < 32 ? 8 : p.vec == 8 && g == 512 ? 32 : 16) / p.vec;
     if (g * p.vec * most < width) continue;
     p.group = g;
     p.nv = p.vec == 1 ? 2 : 1;
@@ -574,14 +616,16 @@ LnPlan ln_plan(int64_t rows, int width, int type, bool aligned, int kept_size) {
     break;
   }
   int blocks = p.group == 0 || p.group == 256 ? 2 : p.group <= 128 ? kLnBwdBlocks<128> : 1;
-  if (kept_size == 0 && p.group > 0) blocks = p.group <= 128 ? kLnFwdBlocks<128> : p.group == 256 ? kLnFwdBlocks<256> : 1;
+  if (kept_size == 0 && p.group > 0)
+    blocks = p.group <= 32 ? kLnFwdBlocks<32> : p.group == 128 ? kLnFwdBlocks<128> : p.group == 256 ? kLnFwdBlocks<256> : 1;
   if (p.vec > 1 && p.group >= 128 && (kept_size != 1 || width % 16 == 0)) {  // bulk copies move multiples of 16 bytes
-    const int64_t bytes = int64_t(width) * (size + kept_size), params = p.group == 1024 ? width * (kept_size ? 4 : 8) : 0;
-    const int64_t fit = ((p.group == 1024 ? 210 << 10 : 160 << 10) - params) / (blocks * bytes);
+    const bool shared = p.group == 1024 || p.vec * p.nv == 32;
+    const int64_t bytes = int64_t(width) * (size + kept_size), params = shared ? width * (kept_size ? 4 : 8) : 0;
+    const int64_t fit = ((shared ? 210 << 10 : 160 << 10) - params) / (blocks * bytes);
     p.slots = int(fit > kLnMaxSlots ? kLnMaxSlots : fit);
     if (p.slots < 2) p.group = p.slots = 0, blocks = 2;
   }
-  const int64_t most_blocks = p.group == 32 ? (rows + 3) / 4 : rows;
+  const int64_t most_blocks = p.group && p.group <= 32 ? (rows * p.group + 127) / 128 : rows;
   p.grid = int(most_blocks < kLnSms * blocks ? most_blocks : kLnSms * blocks);
   return p;
 }
@@ -589,7 +633,7 @@ LnPlan ln_plan(int64_t rows, int width, int type, bool aligned, int kept_size) {
 template <typename T, int VEC, int G, int NV>
 int ln_fwd(const LnPlan& p, const void* x, int64_t xs, const void* w, const void* b, int pt, void* y, float* mean,
            float* rstd, uint8_t* codes, int64_t rows, int width, float eps, cudaStream_t s) {
-  const size_t smem = size_t(p.slots) * width * sizeof(T) + (kLnParamsShared<G> ? size_t(width) * 8 : 0);
+  const size_t smem = size_t(p.slots) * width * sizeof(T) + (kLnParamsShared<VEC, G, NV> ? size_t(width) * 8 : 0);
   if (smem > 40 << 10)  // with the static part it may pass the 48 KB a launch has without asking
     if (int rc = want_smem(layer_norm_fwd_kernel<T, VEC, G, NV>, smem, "layer_norm_fwd")) return rc;
   layer_norm_fwd_kernel<T, VEC, G, NV><<<p.grid, RowShape<T, VEC, G, NV>::kThreads, smem, s>>>(
@@ -600,7 +644,7 @@ template <typename T, int VEC, int G, int NV, bool kCodes, bool kStream>
 int ln_bwd_of(const LnPlan& p, const void* dy, const void* x, int64_t xs, const uint8_t* codes, const float* mean,
               const float* rstd, const void* w, int pt, void* dx, float* partial, int64_t rows, int width, cudaStream_t s) {
   const size_t row = size_t(width) * (sizeof(T) + (kCodes ? 1 : sizeof(T)));
-  const size_t smem = p.slots * row + (kLnParamsShared<G> ? size_t(width) * 4 : 0);
+  const size_t smem = p.slots * row + (kLnParamsShared<VEC, G, NV> ? size_t(width) * 4 : 0);
   if (smem > 40 << 10)
     if (int rc = want_smem(layer_norm_bwd_kernel<T, VEC, G, NV, kCodes, kStream>, smem, "layer_norm_bwd")) return rc;
   layer_norm_bwd_kernel<T, VEC, G, NV, kCodes, kStream><<<p.grid, RowShape<T, VEC, G, NV>::kThreads, smem, s>>>(
@@ -625,8 +669,10 @@ int ln_bwd(const LnPlan& p, const void* dy, const void* x, int64_t xs, const uin
 #define MEK_LN_SHAPES(T, VEC, CALL)                                                          \
   do {                                                                                       \
     if constexpr (VEC == 1) {                                                                \
-      if (p.group == 32 && p.nv == 2) return CALL(T, 1, 32, 2);                              \
-      if (p.group == 32 && p.nv == 4) return CALL(T, 1, 32, 4);                              \
+      if (p.group == 8 && p.nv == 2) return CALL(T, 1, 8, 2);                                \
+      if (p.group == 8 && p.nv == 4) return CALL(T, 1, 8, 4);                                \
+      if (p.group == 8 && p.nv == 8) return CALL(T, 1, 8, 8);                                \
+      if (p.group == 16 && p.nv == 8) return CALL(T, 1, 16, 8);                              \
       if (p.group == 32 && p.nv == 8) return CALL(T, 1, 32, 8);                              \
       if (p.group == 128 && p.nv == 4) return CALL(T, 1, 128, 4);                            \
       if (p.group == 128 && p.nv == 8) return CALL(T, 1, 128, 8);                            \
@@ -636,18 +682,26 @@ int ln_bwd(const LnPlan& p, const void* dy, const void* x, int64_t xs, const uin
       if (p.group == 1024 && p.nv == 16) return CALL(T, 1, 1024, 16);                        \
     } else {                                                                                 \
       constexpr int kMost = 16 / VEC;                                                        \
-      if (p.group == 32 && p.nv == 1) return CALL(T, VEC, 32, 1);                            \
+      if (p.group == 8 && p.nv == 1) return CALL(T, VEC, 8, 1);                              \
       if (p.group == 32 && p.nv == 2) return CALL(T, VEC, 32, 2);                            \
       if (p.group == 128 && p.nv == 2) return CALL(T, VEC, 128, 2);                          \
       if constexpr (VEC == 4) {                                                              \
+        if (p.group == 8 && p.nv == 2) return CALL(T, VEC, 8, 2);                            \
+        if (p.group == 16 && p.nv == 2) return CALL(T, VEC, 16, 2);                          \
         if (p.group == 32 && p.nv == 4) return CALL(T, VEC, 32, 4);                          \
         if (p.group == 128 && p.nv == 4) return CALL(T, VEC, 128, 4);                        \
       } else {                                                                               \
+        if (p.group == 16 && p.nv == 1) return CALL(T, VEC, 16, 1);                          \
+        if (p.group == 32 && p.nv == 1) return CALL(T, VEC, 32, 1);                          \
         if (p.group == 128 && p.nv == 1) return CALL(T, VEC, 128, 1);                        \
       }                                                                                      \
       if (p.group == 256 && p.nv == kMost) return CALL(T, VEC, 256, kMost);                  \
       if (p.group == 512 && p.nv == kMost) return CALL(T, VEC, 512, kMost);                  \
-      if (p.group == 1024 && p.nv == kMost) return CALL(T, VEC, 1024, kMost);                \
+      if constexpr (VEC == 4) {                                                              \
+        if (p.group == 1024 && p.nv == 4) return CALL(T, VEC, 1024, 4);                      \
+      } else {                                                                               \
+        if (p.group == 512 && p.nv == 4) return CALL(T, VEC, 512, 4);                        \
+      }                                                                                      \
     }                                                                                        \
   } while (0)
 

@@ -101,33 +101,56 @@ __device__ __forceinline__ void store_param(void* p, int type, int64_t i, float 
 }
 
 // e4m3 codes (4 exponent bits, 3 mantissa bits, largest 448, NaN but no infinity), rounded to nearest even: off by at
-// most 2^-4 of the value for magnitudes in [2^-6, 448], by 2^-10 below.
+// most 2^-4 of the value for magnitudes in [2^-6, 448], by 2^-10 below.  N of them, in whole words where there are that
+// many (a register a byte otherwise).
 template <int N>
-__device__ __forceinline__ Vec<uint8_t, N> to_e4m3(const float (&v)[N]) {
-  Vec<uint8_t, N> out;
-  if constexpr (N == 1) {
-    out.e[0] = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
-  } else {
+struct Codes {
+  static_assert(N % 4 == 0, "words");
+  uint32_t word[N / 4];
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const __nv_fp8x2_storage_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
-      out.e[i] = uint8_t(two & 0xff), out.e[i + 1] = uint8_t(two >> 8);
-    }
+    for (int i = 0; i < N / 4; ++i) word[i] = 0;
   }
-  return out;
+};
+template <>
+struct Codes<1> {
+  uint8_t byte;
+  __device__ __forceinline__ void clear() { byte = 0; }
+};
+template <int N>
+__device__ __forceinline__ Codes<N> load_codes(const uint8_t* p) {
+  Codes<N> c;
+  if constexpr (N == 1) c.byte = *p;
+  else if constexpr (N == 4) c.word[0] = *reinterpret_cast<const uint32_t*>(p);
+  else {
+    static_assert(N == 8, "one access");
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    c.word[0] = w.x, c.word[1] = w.y;
+  }
+  return c;
 }
 template <int N>
-__device__ __forceinline__ void from_e4m3(const Vec<uint8_t, N>& codes, float (&v)[N]) {
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[N]) {
   if constexpr (N == 1) {
-    v[0] = __half2float(__half(__nv_cvt_fp8_to_halfraw(codes.e[0], __NV_E4M3)));
+    *p = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
   } else {
+    uint32_t word[N / 4];
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const __nv_fp8x2_storage_t two = __nv_fp8x2_storage_t(codes.e[i] | (codes.e[i + 1] << 8));
-      const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
-      v[i] = f.x, v[i + 1] = f.y;
-    }
+    for (int i = 0; i < N / 4; ++i)
+      word[i] = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i], v[4 * i + 1]), __NV_SATFINITE, __NV_E4M3)) |
+                uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2], v[4 * i + 3]), __NV_SATFINITE, __NV_E4M3)) << 16;
+    if constexpr (N == 4) *reinterpret_cast<uint32_t*>(p) = word[0];
+    else *reinterpret_cast<uint2*>(p) = make_uint2(word[0], word[1]);
   }
+}
+// Codes 2 q and 2 q + 1.
+template <int N>
+__device__ __forceinline__ float2 code_pair(const Codes<N>& c, int q) {
+  const __nv_fp8x2_storage_t two = __nv_fp8x2_storage_t(c.word[q / 2] >> (q % 2 * 16));
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(two, __NV_E4M3)));
+}
+__device__ __forceinline__ float code_value(uint8_t code) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
 }
 
 // mbar_wait for copies that are on their way as a rule: the first looks go without the timer, whose reading costs more than
