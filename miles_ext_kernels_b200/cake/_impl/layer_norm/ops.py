@@ -11,7 +11,8 @@ Per row of ``x [..., C]`` (BF16, FP16 or FP32) with a weight and a bias ``[C]``,
 The autograd node keeps ``x`` and two FP32 statistics a row, or, with ``checkpoint="e4m3"``, the rows of ``unit`` as
 e4m3 codes and one statistic: half the bytes of a BF16 ``x``, for gradients that take ``unit`` rounded to 3 mantissa
 bits (off by at most 2^-4 of the value; ``|unit| <= sqrt(C)``, so the codes need no scale).  ``y`` does not change.  The
-parameter gradients are summed in FP32 per block and in FP64 across the blocks, in an order fixed by the extents.
+parameter gradients are summed in FP32 per block and in FP64 across the blocks, in an order fixed by the extents and by
+whether the rows start on 16-byte boundaries.
 """
 
 from __future__ import annotations
@@ -141,7 +142,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     """Autograd-enabled LayerNorm over the last dimension of ``x [..., C]``; returns ``y`` of ``x``'s shape and type.
 
     ``x``: BF16, FP16 or FP32 on a B200, read in place when its rows have unit stride inside and one stride between
-    them, else copied once (the same bits either way).  ``weight``, ``bias``: ``[C]``, each optional, both of one type
+    them, else copied once.  ``weight``, ``bias``: ``[C]``, each optional, both of one type
     out of the three, which their gradients have too.  ``checkpoint``: ``None`` keeps ``x`` for the backward, ``"e4m3"``
     keeps the normalised rows in 8 bits instead (``C`` up to 200,704).  Not twice differentiable."""
     keep = checkpoint_format(OP, checkpoint)

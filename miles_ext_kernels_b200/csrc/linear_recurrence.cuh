@@ -468,6 +468,8 @@ struct Edges {
   int kind;                     // kInside: no boundary, all live; kOneEdge: at most one start and one end
   int start, end;               // of kOneEdge: their tokens, or -1
   int start_seq, end_seq;
+  // a warp behind the last token
+  __device__ __forceinline__ Edges() : starts(0), ends(0), live(0), kind(kInside), start(-1), end(-1), start_seq(0), end_seq(0) {}
   __device__ __forceinline__ Edges(const Sequences& s, const Span& span, int b, int t0) {
     const int n = min(max(s.tokens - t0, 0), kGlrTokens);
     auto below = [](int k) { return k >= 32 ? 0xffffffffu : k <= 0 ? 0u : (1u << k) - 1; };

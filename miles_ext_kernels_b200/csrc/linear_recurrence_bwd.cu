@@ -28,8 +28,9 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   X* ds = reinterpret_cast<X*>(smem + kGlrWarps * (kGlrDecays + kGlrBox<X>) + warp * kGlrBox<X>);
   G* gs = gates_of<G>(decay);
   bool arrived = true;
+  const bool any = t0 < s.tokens;  // a warp behind the last token only takes part in the block's barriers
   if constexpr (kTma) {
-    if (lane == 0) {
+    if (lane == 0 && any) {
       mbar_arrive_expect(&sh.arrived[warp], 2 * kGlrBox<X> + kGlrBox<G>);
       box_load(gs, &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(ds, &dy_map, at.c0, t0, at.b, &sh.arrived[warp]);
@@ -42,7 +43,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
         box_prefetch(&x_map, next.c0, t, next.b);
       }
     }
-  } else {
+  } else if (any) {
     plain_load(gs, p.g, s, at, t0);
     plain_load(ds, p.dy, s, at, t0);
     plain_load(xs, p.x, s, at, t0);
@@ -53,14 +54,16 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
     const Words v = load_words<kTma>(words_at(const_cast<float*>(p.states), s, at, at.tile - 1), s, at);
     h = two(v.B0, v.B1);
   }
-  const Edges edges(s.seq, span_of(s.seq, t0), at.b, t0);
+  const Edges edges = any ? Edges(s.seq, span_of(s.seq, t0), at.b, t0) : Edges();
   const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
   const Two d1 = edges.end >= 0 ? load_state<kTma>(p.d_final, s, at, edges.end_seq) : two(0.f);
-  if constexpr (kTma) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
+  if (kTma && any) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
   {
-    Two A, B, D;
-    if (edges.kind == kInside) walk_tokens<X, G, true, false>(decay, xs, ds, edges, s0, d1, A, B, D);
-    else walk_tokens<X, G, true, true>(decay, xs, ds, edges, s0, d1, A, B, D);
+    Two A = two(1.f), B = two(0.f), D = two(0.f);
+    if (any) {
+      if (edges.kind == kInside) walk_tokens<X, G, true, false>(decay, xs, ds, edges, s0, d1, A, B, D);
+      else walk_tokens<X, G, true, true>(decay, xs, ds, edges, s0, d1, A, B, D);
+    }
     Two R = A;
     if (edges.kind == kManyEdges) {
       if (edges.starts) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
@@ -89,6 +92,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   for (int w = kGlrWarps - 1; w > 0; --w)
     if (w > warp) c = folded(sh.pair[1][w][lane], c);
   if (!arrived) c = two(__int_as_float(0x7fffffff));
+  if (!any) return;
   // forward once more for the state before every token, then back with the adjoint; dx takes dy's place, dg the gates'
   Two before[kGlrTokens];
   if (edges.kind == kInside) {
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   if constexpr (kTma) {
     fence_async_smem();
     __syncwarp();
-    if (lane == 0 && t0 < s.tokens) {
+    if (lane == 0) {
       box_store(&dx_map, at.c0, t0, at.b, ds);
       box_store(&dg_map, at.c0, t0, at.b, gs);
       tma_store_commit();

@@ -22,8 +22,9 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   float* decay = reinterpret_cast<float*>(smem + warp * kGlrDecays);
   X* xs = reinterpret_cast<X*>(smem + kGlrWarps * kGlrDecays + warp * kGlrBox<X>);
   bool arrived = true;
+  const bool any = t0 < s.tokens;  // a warp behind the last token only takes part in the block's barriers
   if constexpr (kTma) {
-    if (lane == 0) {
+    if (lane == 0 && any) {
       mbar_arrive_expect(&sh.arrived[warp], kGlrBox<X> + kGlrBox<G>);
       box_load(gates_of<G>(decay), &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(xs, &x_map, at.c0, t0, at.b, &sh.arrived[warp]);
@@ -33,17 +34,20 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
         box_prefetch(&x_map, next.c0, next.tile * kGlrTile + warp * kGlrTokens, next.b);
       }
     }
-  } else {
+  } else if (any) {
     plain_load(gates_of<G>(decay), p.g, s, at, t0);
     plain_load(xs, p.x, s, at, t0);
     __syncwarp();
   }
-  const Edges edges(s.seq, span_of(s.seq, t0), at.b, t0);
+  const Edges edges = any ? Edges(s.seq, span_of(s.seq, t0), at.b, t0) : Edges();
   const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
-  if constexpr (kTma) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
-  Two A, B, none;
-  if (edges.kind == kInside) walk_tokens<X, G, false, false>(decay, xs, xs, edges, none, none, A, B, none);
-  else walk_tokens<X, G, false, true>(decay, xs, xs, edges, s0, none, A, B, none);
+  if (kTma && any) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
+  const Two none = two(0.f);
+  Two A = two(1.f), B = none, no_adjoint;
+  if (any) {
+    if (edges.kind == kInside) walk_tokens<X, G, false, false>(decay, xs, xs, edges, none, none, A, B, no_adjoint);
+    else walk_tokens<X, G, false, true>(decay, xs, xs, edges, s0, none, A, B, no_adjoint);
+  }
   if (edges.kind == kManyEdges) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
   if (edges.starts) A = two(kGlrReset);
   if (!arrived) A = two(kGlrReset), B = two(__int_as_float(0x7fffffff));
@@ -63,6 +67,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   for (int w = 0; w < kGlrWarps - 1; ++w)
     if (w < warp) h = folded(sh.pair[0][w][lane], h);
   if (!arrived) h = two(__int_as_float(0x7fffffff));
+  if (!any) return;
   if (edges.kind == kInside) {
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) {
@@ -94,7 +99,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   if constexpr (kTma) {
     fence_async_smem();
     __syncwarp();
-    if (lane == 0 && t0 < s.tokens) {
+    if (lane == 0) {
       box_store(&y_map, at.c0, t0, at.b, xs);
       tma_store_commit();
       tma_store_wait_read();

@@ -246,6 +246,38 @@ def test_empty_rows_missing_parameters_and_partial_gradients():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_offsets_past_32_bits(checkpoint):
+    """2.2 G elements a tensor: the last rows against the same rows on their own."""
+    rows, width = 540_672, 4096
+    x = torch.empty(rows, width, device="cuda", dtype=BF16).normal_()
+    dy = torch.empty_like(x).normal_()
+    w, b = torch.randn(width, device="cuda").to(BF16), torch.randn(width, device="cuda").to(BF16)
+    assert x.numel() > 1 << 31
+    got = run(x, w, b, dy, checkpoint=checkpoint)
+    tail = run(x[-300:], w, b, dy[-300:], checkpoint=checkpoint)
+    for name in ("y", "dx"):
+        assert torch.equal(got[name][-300:], tail[name]), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 4097])
+def test_rows_side_by_side_in_a_warp(rows, dtype):
+    """Narrow rows share warps; the last warp's places may be empty, and a row's neighbours do not reach it."""
+    for width in (3, 24, 64, 100, 128):
+        x, w, b, dy = make(rows, width, dtype, FP32, seed=9)
+        got = run(x, w, b, dy)
+        check(got, x, w, b, dy, what=f"{rows} x {width}")
+        if rows > 2:
+            x[1] = float("nan")
+            bad = run(x, w, b, dy)
+            others = [r for r in range(rows) if r != 1]
+            assert torch.equal(bad["y"][others], got["y"][others]) and torch.equal(bad["dx"][others], got["dx"][others])
+            assert torch.equal(bad["db"], got["db"]) and bad["dw"].isnan().all()
+
+
+@pytest.mark.gpu
 def test_against_differences_of_the_forward():
     x, w, b, dy = make(3, 37, FP32, FP32, seed=6)
     got = run(x, w, b, dy)

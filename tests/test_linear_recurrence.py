@@ -351,6 +351,49 @@ def test_other_streams_the_pool_and_captured_graphs():
         assert all(torch.equal(out[n].detach(), want[n]) for n in want)
 
 
+@pytest.mark.gpu
+def test_time_major_operands_and_a_backward_run_twice():
+    """[T, B, C] memory behind [B, T, C] views: the token stride is the larger one."""
+    from miles_ext_kernels_b200.cake.linear_recurrence import gated_linear_recurrence
+
+    x, g, h0, dy, dl = make(3, 300, 128, BF16, BF16, 3, seed=13)
+    want = run(x, g, h0, dy, dl)
+    views = [t.transpose(0, 1).contiguous().transpose(0, 1) for t in (x, g, dy)]
+    assert views[0].stride(0) == 128 and views[0].stride(1) == 3 * 128
+    got = run(views[0], views[1], h0, views[2], dl)
+    assert all(torch.equal(got[n], want[n]) for n in want)
+    leaves = [t.clone().requires_grad_() for t in (x, g, h0)]
+    outs = gated_linear_recurrence(*leaves, output_final_state=True)
+    for _ in range(2):
+        grads = torch.autograd.grad(outs, leaves, (dy, dl), retain_graph=True)
+        assert all(torch.equal(a, want[n]) for a, n in zip(grads, ("dx", "dg", "dh0")))
+
+
+@pytest.mark.gpu
+def test_many_chains_and_many_short_sequences():
+    """More chains than blocks (one warp looks back), batches of one tile, a batch of two tokens."""
+    for batch, tokens, channels in ((40, 300, 1024), (300, 100, 64), (700, 2, 192)):
+        x, g, h0, dy, dl = make(batch, tokens, channels, BF16, FP32, batch, seed=14)
+        got = run(x, g, h0, dy, dl)
+        for rows in (slice(0, 2), slice(batch - 2, batch)):
+            part = {n: t[rows] for n, t in got.items()}
+            check(part, x[rows], g[rows], h0[rows], dy[rows], dl[rows], [tokens] * 2, f"{batch} x {tokens} x {channels}")
+        again = run(x, g, h0, dy, dl)
+        assert all(torch.equal(got[n], again[n]) for n in got)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """2.2 G elements a tensor; closed gates make the last tokens independent of the ones before."""
+    tokens, channels = 540_672, 4096
+    x = torch.empty(1, tokens, channels, device="cuda", dtype=BF16).normal_()
+    g = torch.full((1, tokens, channels), -200.0, device="cuda", dtype=BF16)
+    dy = torch.empty_like(x).normal_()
+    assert x.numel() > 1 << 31
+    got = run(x, g, None, dy, None, final=False)
+    assert torch.equal(got["y"], x) and torch.equal(got["dx"], dy) and got["dg"].abs().max() == 0
+
+
 # ---- the single-token step -------------------------------------------------------------------------------------------
 def step_reference(x, g, state, slots):
     """Row after row in 64 bits: ``(y, state, y slack, state slack)``."""
@@ -413,6 +456,18 @@ def test_the_step_continues_a_sequence_and_reads_strided_rows():
     assert step(x[:0, 0], g[:0, 0], pool).shape == (0, 96)
     with pytest.raises(ValueError, match="dense inside its slot"):
         step(x[:, 0], g[:, 0], torch.zeros(96, 6, device="cuda").t(), slots)
+
+
+@pytest.mark.gpu
+def test_the_step_on_a_pool_past_32_bits():
+    from miles_ext_kernels_b200.cake.linear_recurrence import gated_linear_recurrence_step as step
+
+    pool = torch.zeros(540_000, 4096, device="cuda")
+    assert pool.numel() > 1 << 31
+    x, g, _, _, _ = make(1, 3, 4096, BF16, FP32, 1, seed=15)
+    slots = torch.tensor([539_999, 3, 530_001], device="cuda")
+    y = step(x[0], g[0], pool, slots)
+    assert torch.equal(y, x[0]) and torch.equal(pool[slots].to(BF16), x[0]) and int((pool != 0).any(1).sum()) == 3
 
 
 @pytest.mark.gpu
