@@ -239,6 +239,11 @@ def option(op: str | None, dest: str) -> Any:
     return _Process.settings.get(dest, defaults[dest])
 
 
+def pool_bytes() -> int:
+    """``option(None, "cake_workspace_pool_bytes")``, read on the way to every scratch buffer."""
+    return _Process.settings.get("cake_workspace_pool_bytes", 0)
+
+
 def warn_runs_det(op: str, reason: str) -> None:
     """Log, once per ``(op, reason)``, that a call the ``fast`` variant does not serve runs ``det``."""
     seen = (op, reason)

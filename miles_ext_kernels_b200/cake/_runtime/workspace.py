@@ -53,10 +53,12 @@ def _locate(device: Any) -> tuple[Any, Any]:
     """``(pool key, torch.device)``: the CUDA index (current device for a bare ``"cuda"``), else the device name."""
     import torch
 
-    where = torch.device(device)
+    where = device if isinstance(device, torch.device) else torch.device(device)
     if where.type != "cuda":
         return str(where), where
-    index = where.index if where.index is not None else torch.cuda.current_device()
+    if where.index is not None:
+        return where.index, where
+    index = torch.cuda.current_device()
     return index, torch.device("cuda", index)
 
 
@@ -77,7 +79,7 @@ def take(op: str, role: str, shape: Sequence[int], dtype: Any, device: Any) -> A
     ``(op, role)`` on the current stream, or a plain ``torch.empty`` when the pool does not serve the request."""
     import torch
 
-    bound = config.option(None, "cake_workspace_pool_bytes")
+    bound = config.pool_bytes()
     key, where = _locate(device)
     with _lock:
         pool = _pools.setdefault(key, _DevicePool())

@@ -476,16 +476,18 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
   }
 }
 
-// Column sums of partial [blocks, 2, width] in block order, FP64: 32 columns a block, eight runs of blocks.
-__global__ void __launch_bounds__(256) layer_norm_param_grad_kernel(const float* __restrict__ partial, int blocks,
-                                                                    int width, void* __restrict__ dw,
-                                                                    void* __restrict__ db, int param_type) {
-  __shared__ double s[8][32];
+// Column sums of partial [blocks, 2, width] in block order, FP64: 32 columns a block, a warp per run of blocks, so that few
+// additions wait for one another (32,768 x 4,096 bf16: the backward 156.5 us with eight runs, 153.5 with 32).
+constexpr int kLnRuns = 32;
+__global__ void __launch_bounds__(32 * kLnRuns) layer_norm_param_grad_kernel(const float* __restrict__ partial, int blocks,
+                                                                             int width, void* __restrict__ dw,
+                                                                             void* __restrict__ db, int param_type) {
+  __shared__ double s[kLnRuns][32];
   const int column = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + column;
   void* out = blockIdx.y ? db : dw;
   if (out == nullptr) return;  // uniform over the block
-  const int per = (blocks + 7) / 8, lo = run * per, hi = min(lo + per, blocks);
+  const int per = (blocks + kLnRuns - 1) / kLnRuns, lo = run * per, hi = min(lo + per, blocks);
   double sum = 0.0;
   if (c < width) {
     const float* p = partial + int64_t(blockIdx.y) * width + c;
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(256) layer_norm_param_grad_kernel(const float*
   __syncthreads();
   if (run == 0 && c < width) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) sum += s[k][column];
+    for (int k = 1; k < kLnRuns; ++k) sum += s[k][column];
     store_param(out, param_type, c, float(sum));
   }
 }
@@ -806,7 +808,7 @@ int mek_layer_norm_bwd(const void* dy, const void* x, int type, const uint8_t* c
   };
   if (int rc = main_launch()) return rc;
   if (partial) {
-    layer_norm_param_grad_kernel<<<dim3((w + 31) / 32, 2), 256, 0, s>>>(partial, p.grid, w, dw, db, param_type);
+    layer_norm_param_grad_kernel<<<dim3((w + 31) / 32, 2), 32 * kLnRuns, 0, s>>>(partial, p.grid, w, dw, db, param_type);
     return launched("layer_norm_bwd (parameters)");
   }
   return MEK_OK;
