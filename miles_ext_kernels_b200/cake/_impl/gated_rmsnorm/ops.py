@@ -160,7 +160,9 @@ def rmsnorm_silu_gate(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, ep
     the gradients).  ``y`` does not
     change."""
     config.variant(OP)  # both variants run the same kernels; an unknown configuration still raises here
-    return _RmsnormSiluGate.apply(x, z, weight, eps, checkpoint_format(OP, checkpoint))
+    keep = checkpoint_format(OP, checkpoint) and torch.is_grad_enabled() and (
+        x.requires_grad or z.requires_grad or weight.requires_grad)
+    return _RmsnormSiluGate.apply(x, z, weight, eps, keep)
 
 
 def prebuild(*, device: Any = None, max_workers: int | None = None) -> list[Path]:

@@ -134,9 +134,10 @@ class Entry:
 
     def __call__(self, device: torch.device, *arguments: Any) -> None:
         lib = _library
-        if lib is None or lib is not self._owner:
-            lib = self._owner = library()
+        if lib is None or lib is not self._owner:  # the owner last: autograd's thread may look while this one binds
+            lib = library()
             self._call = ctypes.CFUNCTYPE(ctypes.c_int, *self._types)((f"mek_{self._name}", lib._dll))
+            self._owner = lib
         index = device.index
         stream = torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
         log = _log

@@ -13,7 +13,8 @@
 // 8-bit checkpoint: the forward may also write what the backward needs as e4m3 codes -- the normalised row n = x rstd,
 // whose values stay below sqrt(128) and need no scale, and z under one power of two a row (exact to divide by, so
 // the code's rounding is the only error) -- and the backward read them in the place of x and z: 2 bytes an element kept
-// instead of 4.
+// instead of 4.  1,048,576 rows: forward 217 us = 4.9 TB/s, backward 238 us = 4.5 TB/s (copy: 6.5), bound by instructions
+// (67 - 70 % of the issue slots: two MUFU operations and about 20 others an element).
 #include "common.cuh"
 #include "rowio.cuh"
 #include "umma.cuh"

@@ -7,8 +7,15 @@
 // barrier a row instead of two.
 //
 // The weight and bias gradients: a thread owns the same columns in every row of its block and sums them in FP32
-// registers; a second launch adds the blocks' sums in FP64 in block order.  The grid is a function of the extents
-// alone, so identical inputs give identical bits.
+// registers; a second launch adds the blocks' sums in FP64 in a fixed order.  The grid is a function of the extents and
+// of the rows' alignment, so identical inputs give identical bits.
+//
+// Arithmetic on packed pairs of FP32 (half the instructions; a row of 16 elements a thread took 427 of them scalar, which
+// bounded it), rows of a whole block streamed by bulk copies, narrow rows side by side in a warp.  Measured, bf16:
+// 32,768 x 4,096 forward 107 us = 5.0 TB/s, backward 154 us = 5.2 TB/s with the last sums (copy: 6.5); 16,384 x 8,192
+// with the checkpoint 135 + 140 us; 65,536 x 2,048 96 + 150.  What bounds it: the chain of a row's phases (wait, sums,
+// shuffles, barrier, output) with three blocks an SM (backward: two), at 60 % of the issue slots; below 512 columns the
+// instructions of a row.
 //
 // 8-bit checkpoint: the forward may also write unit as e4m3 codes and the backward read them in the place of x and
 // mean.  |unit| <= sqrt(C), so up to 448^2 = 200,704 columns the codes need no scale.
@@ -259,11 +266,11 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
   }
   __syncthreads();
   int slot = 0, parity = 0, phase = 0;
+  bool failed = false;  // a wait ran out: the rows from there on are NaN, and nothing waits again
   auto one_row = [&](int64_t r, RowPart<T, VEC, G, NV>& part) {
     const bool live = Shape::kSide == 1 || r < rows;  // rows side by side in a warp go through its shuffles together
-    bool arrived = true;
     if constexpr (kStream) {
-      arrived = mbar_wait_soon(&s_full[slot], parity);
+      if (!failed) failed = !mbar_wait_soon(&s_full[slot], parity);
       part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
     }
     Two xv[kPairs], sum = two(0.f);
@@ -274,7 +281,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
     // this warp's mean and squares about it; a mean is rounded before it is subtracted, whether or not it is stored: the
     // same y either way
     float2 s = split(sum);
-    if (!arrived) s.x = __int_as_float(0x7fffffff);
+    if (failed) s.x = __int_as_float(0x7fffffff);
     float total = lane_sum<G>(s.x + s.y);
     float mean = __fmul_rn(total, inv_count);
     Two squares = two(0.f);
@@ -298,7 +305,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
     if constexpr (G > 32) {  // the warps' by Chan's rule
       if (threadIdx.x % 32 == 0) s_part[phase][warp] = make_float2(mean, m2);
       __syncthreads();
-      if (kStream && threadIdx.x == 0 && r + slots * step < rows) {  // everybody has the row in registers
+      if (kStream && threadIdx.x == 0 && !failed && r + slots * step < rows) {  // everybody has the row in registers
         mbar_arrive_expect(&s_full[slot], bytes);
         bulk_load(smem + slot * bytes, x + (r + slots * step) * x_stride, bytes, &s_full[slot]);
       }
@@ -342,6 +349,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
     for (int k = 0; k < kDepth; ++k)
       if (r - side + k * step < rows) one_row(r + k * step, parts[k]);
   }
+  if (kStream && failed) let_copies_land();
 }
 
 // kCodes: unit comes from the 8-bit checkpoint, x and mean are not read.  partial [gridDim.x, 2, width] (or NULL).
@@ -400,15 +408,15 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
   }
   __syncthreads();
   int slot = 0, parity = 0, phase = 0;
+  bool failed = false;
   auto one_row = [&](int64_t r, int k) {
     const bool live = Shape::kSide == 1 || r < rows;
     const float rstd = ahead_rstd[k];
     const Two mean = two(ahead_mean[k]), scale = two(rstd);
-    bool arrived = true;
     RowPart<T, VEC, G, NV> g_part;
     RowPart<Kept, VEC, G, NV> k_part;
     if constexpr (kStream) {
-      arrived = mbar_wait_soon(&s_full[slot], parity);
+      if (!failed) failed = !mbar_wait_soon(&s_full[slot], parity);
       g_part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
       k_part.load(reinterpret_cast<const Kept*>(smem + slot * bytes + dy_bytes), lane, width);
     } else {
@@ -431,8 +439,8 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
       s2 = fma2(dn, u, s2);
     }
     const float2 a = split(s1), c = split(s2);
-    const float2 sums = group_sum<G>(arrived ? a.x + a.y : __int_as_float(0x7fffffff), c.x + c.y, s_part, phase);
-    if (kStream && threadIdx.x == 0 && r + slots * step < rows) fill(slot, r + slots * step);  // all have read the row
+    const float2 sums = group_sum<G>(failed ? __int_as_float(0x7fffffff) : a.x + a.y, c.x + c.y, s_part, phase);
+    if (kStream && threadIdx.x == 0 && !failed && r + slots * step < rows) fill(slot, r + slots * step);  // all have read the row
     const Two m1 = two(sums.x * inv_width), m2 = two(-(sums.y * inv_width));
     if (live) store_row<T, VEC, G, NV>(dx + r * width, lane, width, [&](int q) {
       return mul2(fma2(unit(q), m2, sub2(mul2(g_part.pair(q), w.pair(q, lane)), m1)), scale);
@@ -446,6 +454,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
     for (int k = 0; k < kDepth; ++k)
       if (r - side + k * step < rows) one_row(r + k * step, k);
   }
+  if (kStream && failed) let_copies_land();
   if (partial == nullptr) return;
   float* mine = partial + int64_t(blockIdx.x) * 2 * width;
   if constexpr (Shape::kRows == 1) {
@@ -503,7 +512,9 @@ __global__ void __launch_bounds__(32 * kLnRuns) layer_norm_param_grad_kernel(con
   }
 }
 
-// ---- rows too wide for one block's registers: the row is read again for every pass (from L2) ----------------------
+// ---- rows too wide for one block (16-bit: over 16,384 columns; FP32: over 13,440 forward, 10,752 backward, whose parameters
+// and two rows in flight no longer fit the shared memory): the row is read again for every pass, from L2 (4,096 x 20,000
+// bf16: forward 183 us, backward 462).
 constexpr int kWideThreads = 1024;
 __device__ __forceinline__ float2 wide_sum(float2 v, float2* s) {
   v.x = warp_sum(v.x), v.y = warp_sum(v.y);

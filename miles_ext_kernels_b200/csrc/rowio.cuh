@@ -161,6 +161,12 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
   return mbar_wait(bar, parity);
 }
 
+// After a wait that ran out: copies that are still in flight may write to this block's shared memory.
+__device__ __forceinline__ void let_copies_land() {
+  const uint64_t t0 = global_timer_ns();
+  while (global_timer_ns() - t0 < 100000) __nanosleep(1000);
+}
+
 __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
   for (int m = 16; m >= 1; m >>= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
