@@ -6,7 +6,7 @@ Per channel, with ``a = exp(g)`` and the state of a sequence starting at ``h0`` 
     h[t] = a[t] h[t-1] + x[t],   y[t] = h[t]
     dh[t] = dy[t] + a[t+1] dh[t+1],   dx = dh,   dg[t] = dh[t] a[t] h[t-1],   dh0 = a[0] dh[0]
 
-States and sums in FP32, one rounding per output; a decay below e^-87, where FP32 ends, counts as zero.  The autograd node keeps ``x``, ``g`` and the FP32 state after every
+States and sums in FP32, one rounding per output; a decay below e^-87.7, where FP32 ends, counts as zero.  The autograd node keeps ``x``, ``g`` and the FP32 state after every
 tile of 128 tokens; the backward recomputes the states inside a tile, so ``dg`` does not see a rounded ``y``.
 """
 
@@ -197,15 +197,8 @@ def gated_linear_recurrence(
     return y, final
 
 
-def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
-                                 state_indices: torch.Tensor | None = None) -> torch.Tensor:
-    """One token of every row: ``state[i] = exp(g) state[i] + x`` in place; returns the new state as ``y`` in ``x``'s type.
-
-    ``x``: BF16, FP16 or FP32 ``[R, ...]``; ``g``: the log decay in nats, ``x``'s shape, in any of the three types.
-    ``state``: the FP32 pool ``[N, ...]``, dense inside a slot (any stride between them), updated in place, so not for
-    autograd.  ``state_indices``: int32 or int64 ``[R]``, the slot of every row (``None``: row ``r`` uses slot ``r`` and
-    ``N >= R``).  A row whose index is outside ``[0, N)``, -1 for example, is padding: no state changes and its ``y`` is
-    zero.  Rows that name one slot are applied one after the other, in row order."""
+def _explain_step(x, g, state, state_indices):
+    """Raise the ``ValueError`` that says what is wrong with a step's arguments; returns where nothing is."""
     if x.dim() < 2:
         raise ValueError(f"linear_recurrence: x must be [rows, ...channels]; got {tuple(x.shape)}")
     if g.shape != x.shape:
@@ -234,8 +227,31 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
             raise ValueError(f"linear_recurrence: {name} is on {t.device}, x on {x.device}")
     if not x.is_cuda:
         raise ValueError("linear_recurrence: x must be a CUDA tensor")
+
+
+def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.Tensor,
+                                 state_indices: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of every row: ``state[i] = exp(g) state[i] + x`` in place; returns the new state as ``y`` in ``x``'s type.
+
+    ``x``: BF16, FP16 or FP32 ``[R, ...]``; ``g``: the log decay in nats, ``x``'s shape, in any of the three types.
+    ``state``: the FP32 pool ``[N, ...]``, dense inside a slot (any stride between them), updated in place, so not for
+    autograd.  ``state_indices``: int32 or int64 ``[R]``, the slot of every row (``None``: row ``r`` uses slot ``r`` and
+    ``N >= R``).  A row whose index is outside ``[0, N)``, -1 for example, is padding: no state changes and its ``y`` is
+    zero.  Rows that name one slot are applied one after the other, in row order."""
+    device, shape, trailing = x.device, x.shape, state.shape[1:]
+    if not (  # one test for the usual call; _explain_step says what is wrong with any other
+        x.is_cuda and x.dim() == 2 and g.shape == shape and trailing == shape[1:] and state.dtype is torch.float32
+        and x.dtype in TYPES and g.dtype in TYPES and g.device == device and state.device == device
+        and state_indices is not None and state_indices.dtype in (torch.int32, torch.int64)
+        and state_indices.shape == shape[:1] and state_indices.device == device and 0 < shape[1] <= _MAX_CHANNELS
+        and state.shape[0] > 0
+        and not ((x.requires_grad or g.requires_grad or state.requires_grad) and torch.is_grad_enabled())
+    ):
+        _explain_step(x, g, state, state_indices)
+    rows, pool = shape[0], state.shape[0]
+    channels = shape[1:].numel()
     pooled = state
-    if len(trailing) > 1:
+    if state.dim() > 2:
         try:
             pooled = state.view(pool, channels)
         except RuntimeError:
@@ -247,7 +263,6 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
         return y
     xv, gv = _flat_rows(x, channels), _flat_rows(g, channels)
     slots = None if state_indices is None else state_indices.contiguous()
-    device = x.device
     with on_device(device):
         _step(device, xv.data_ptr(), TYPES[x.dtype], gv.data_ptr(), TYPES[g.dtype], pooled.data_ptr(), pointer(slots),
               slots is not None and slots.dtype == torch.int64, y.data_ptr(), rows, pool, channels, xv.stride(0),

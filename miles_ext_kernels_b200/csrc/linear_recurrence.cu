@@ -40,8 +40,10 @@ __global__ void __launch_bounds__(256) glr_step_kernel(const X* __restrict__ x, 
       const bool same = int64_t(slots[k]) == slot;
       before |= same && k < r, again |= same && k > r;
     }
-    if (__syncthreads_or(before)) return;
-    again = __syncthreads_or(again);
+    if (__syncthreads_or(before || again)) {  // as a rule no two rows share a slot
+      if (__syncthreads_or(before)) return;
+      again = __syncthreads_or(again);
+    }
   }
   if (!mine) return;
   unpack(hr, h);
