@@ -459,6 +459,23 @@ def test_the_step_continues_a_sequence_and_reads_strided_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,gdtype", [(BF16, FP32), (FP32, FP16)])
+@pytest.mark.parametrize("channels", [2056, 2060])
+def test_a_large_step_with_wide_and_narrow_accesses(channels, dtype, gdtype):
+    from miles_ext_kernels_b200.cake.linear_recurrence import gated_linear_recurrence_step as step
+
+    rows, pool = 530, 600
+    x, g, _, _, _ = make(1, rows, channels, dtype, gdtype, 1, seed=16)
+    state = torch.randn(pool, channels, device="cuda")
+    order = torch.randperm(pool, generator=torch.Generator().manual_seed(4))[:rows]
+    order[7], order[300], order[529], order[8] = order[2], order[2], order[100], -1
+    pooled = state.clone()
+    y = step(x[0], g[0], pooled, order.cuda())
+    ref = step_reference(x[0], g[0], state, order.tolist())
+    assert R.misses(y, ref[0], ref[2]) == 0 and R.misses(pooled, ref[1], ref[3]) == 0
+
+
+@pytest.mark.gpu
 def test_the_step_on_a_pool_past_32_bits():
     from miles_ext_kernels_b200.cake.linear_recurrence import gated_linear_recurrence_step as step
 
