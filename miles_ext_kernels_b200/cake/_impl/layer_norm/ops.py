@@ -61,6 +61,8 @@ def _check_width(width: int, keep: bool) -> None:
 def _rows_of(x: torch.Tensor) -> torch.Tensor:
     """``x`` as ``[rows, C]`` with unit stride inside a row: read in place where the leading dimensions merge to one
     row stride, else copied once."""
+    if x.is_contiguous() and x.dim() == 2:
+        return x
     width = x.shape[-1]
     if x.dim() != 2:
         try:
@@ -137,15 +139,8 @@ class _LayerNorm(torch.autograd.Function):
     backward = staticmethod(once_differentiable(_gradients))
 
 
-def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, *,
-               checkpoint: str | None = None) -> torch.Tensor:
-    """Autograd-enabled LayerNorm over the last dimension of ``x [..., C]``; returns ``y`` of ``x``'s shape and type.
-
-    ``x``: BF16, FP16 or FP32 on a B200, read in place when its rows have unit stride inside and one stride between
-    them, else copied once.  ``weight``, ``bias``: ``[C]``, each optional, both of one type
-    out of the three, which their gradients have too.  ``checkpoint``: ``None`` keeps ``x`` for the backward, ``"e4m3"``
-    keeps the normalised rows in 8 bits instead (``C`` up to 200,704).  Not twice differentiable."""
-    keep = checkpoint_format(OP, checkpoint)
+def _explain(x, weight, bias, keep):
+    """Raise the ``ValueError`` that says what is wrong with a call's arguments; returns where nothing is."""
     if x.dim() < 1:
         raise ValueError("layer_norm: x must have at least one dimension")
     width = x.shape[-1]
@@ -163,9 +158,27 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     _check_types(x.dtype, x.dtype if param is None else param.dtype)
     if not x.is_cuda:
         raise ValueError("layer_norm: x must be a CUDA tensor")
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None, eps: float = 1e-5, *,
+               checkpoint: str | None = None) -> torch.Tensor:
+    """Autograd-enabled LayerNorm over the last dimension of ``x [..., C]``; returns ``y`` of ``x``'s shape and type.
+
+    ``x``: BF16, FP16 or FP32 on a B200, read in place when its rows have unit stride inside and one stride between
+    them, else copied once.  ``weight``, ``bias``: ``[C]``, each optional, both of one type out of the three, which their
+    gradients have too.  ``checkpoint``: ``None`` keeps ``x`` for the backward, ``"e4m3"`` keeps the normalised rows in 8
+    bits instead (``C`` up to 200,704).  Not twice differentiable."""
+    keep = checkpoint is not None and checkpoint_format(OP, checkpoint)
+    if not (  # one test for the usual call; _explain says what is wrong with any other
+        weight is not None and bias is not None and x.is_cuda and x.dim() > 0 and x.dtype in TYPES and weight.dtype in TYPES
+        and weight.dtype is bias.dtype and weight.shape == bias.shape == x.shape[-1:]
+        and weight.device == bias.device == x.device and 0 < x.shape[-1] <= _CHECKPOINT_WIDTH
+    ):
+        _explain(x, weight, bias, keep)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
+            ) and torch.is_grad_enabled():
         return _LayerNorm.apply(x, weight, bias, float(eps), keep)
     return _forward(x, weight, bias, float(eps), keep, False)[0]
 
