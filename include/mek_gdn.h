@@ -270,7 +270,7 @@ int mek_qk_grad_finish(const float* x, const void* raw_rows, const float* rstd, 
  *     rstd = 1 / sqrt(mean(x^2) + eps),   y = bf16(((x rstd) weight) silu(z))
  * x, z bf16: row (token, head) at token * token_stride + head * head_stride elements (strides multiples of 8, bases
  * 16-byte aligned; z is usually a column slice of the layer's input projection); weight bf16 [128]; y, dy, dx, dz dense
- * bf16 [rows, 128]; rows = tokens * heads.  The weight gradient (bf16 [128], or NULL with dw_partial NULL) is summed
+ * bf16 [rows, 128]; all of them 16-byte aligned; rows = tokens * heads.  The weight gradient (bf16 [128], or NULL with dw_partial NULL) is summed
  * in a fixed order: per block in FP32 into dw_partial fp32 [mek_gated_rmsnorm_partial_rows(rows), 128], then over the
  * blocks in FP64.  Replaces the reference's `cake_rmsnorm_silu_gate_det_train` package (reference:
  * miles_ext_kernels/cake/_impl/gated_rmsnorm/ops.py:126-148). */

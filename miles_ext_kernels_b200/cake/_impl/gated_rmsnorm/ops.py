@@ -23,7 +23,7 @@ import torch
 from ..._runtime import config, loader, registry, workspace
 from ..gdn import native
 from ..gdn.native import pointer
-from ..rows import checkpoint_format, on_device
+from ..rows import aligned, checkpoint_format, on_device
 
 __all__ = ["check_supported", "prebuild", "release", "rmsnorm_silu_gate"]
 
@@ -107,7 +107,7 @@ class _RmsnormSiluGate(torch.autograd.Function):
             zv, z_heads, zt, zh = _rows_view(z, "z")
             if z_heads != heads:
                 raise ValueError("rmsnorm_silu_gate: x and z must split their rows into the same heads")
-            w = weight.contiguous()
+            w = aligned(weight)
             with on_device(device):
                 (_fwd_keep if keep else _fwd)(device, xv.data_ptr(), zv.data_ptr(), w.data_ptr(), y.data_ptr(),
                                               *(t.data_ptr() for t in kept), rows, heads, xt, xh, zt, zh, float(eps))
@@ -120,14 +120,14 @@ class _RmsnormSiluGate(torch.autograd.Function):
         *kept, weight = ctx.saved_tensors
         device = dy.device
         rows = dy.numel() // HEAD_DIM
-        dy = dy.contiguous() if dy.dtype == torch.bfloat16 else dy.to(torch.bfloat16).contiguous()
+        dy = aligned(dy.to(torch.bfloat16))
         dx, dz = torch.empty_like(dy), torch.empty_like(dy)
         want_dw = ctx.needs_input_grad[2]
         dw = weight.new_empty(HEAD_DIM) if want_dw else None
         if not rows and want_dw:
             dw.zero_()
         if rows:
-            w = weight.contiguous()
+            w = aligned(weight)
             with on_device(device):
                 partial = None
                 if want_dw:

@@ -1,5 +1,5 @@
 """What the row operators (LayerNorm, the gated norm's checkpoint, the linear recurrence) share on the host: element
-types as the C ABI numbers them, checkpoint formats, the device check and the device guard."""
+types as the C ABI numbers them, checkpoint formats, alignment, the device check and the device guard."""
 
 from __future__ import annotations
 
@@ -11,7 +11,7 @@ from torch.autograd.function import once_differentiable as _guarded
 
 from .._runtime import loader
 
-__all__ = ["CHECKPOINTS", "TYPES", "check_device", "checkpoint_format", "on_device", "once_differentiable"]
+__all__ = ["CHECKPOINTS", "TYPES", "aligned", "check_device", "checkpoint_format", "on_device", "once_differentiable"]
 
 # element types of the C ABI
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -26,6 +26,13 @@ def on_device(device: torch.device) -> Any:
     if device.index is None or device.index == torch.cuda.current_device():
         return _NOTHING
     return torch.cuda.device(device)
+
+
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` dense and on a 16-byte boundary, copied once where it is not (a slice of a flat buffer is contiguous and may
+    start anywhere)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def once_differentiable(backward: Any) -> Any:

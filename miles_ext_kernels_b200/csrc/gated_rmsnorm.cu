@@ -311,6 +311,15 @@ int check_norm(const char* what, int64_t rows, int heads, int64_t xt, int64_t xh
   return MEK_OK;
 }
 
+// What the kernels read and write as dense rows, 16 bytes an access.
+int check_dense(const char* what, const void* a, const void* b, const void* c = nullptr, const void* d = nullptr) {
+  using namespace mek;
+  auto bits = [](const void* p) { return reinterpret_cast<uintptr_t>(p); };
+  if ((bits(a) | bits(b) | bits(c) | bits(d)) % 16 != 0)
+    return fail(MEK_ERR_INVALID, "%s: the weight, y, dy, dx and dz must be 16-byte aligned", what);
+  return MEK_OK;
+}
+
 int check_checkpoint(const char* what, const mek::NormCheckpoint& c) {
   using namespace mek;
   if (!c.n_codes || !c.z_codes || !c.z_exponent || !c.rstd) return fail(MEK_ERR_INVALID, "%s: a null pointer", what);
@@ -326,6 +335,7 @@ int norm_fwd(const char* what, const void* x, const void* z, const void* weight,
   if (!x || !z || !weight || !y) return fail(MEK_ERR_INVALID, "%s: a null pointer", what);
   if (int rc = check_norm(what, rows, heads, x_token_stride, x_head_stride, z_token_stride, z_head_stride, x, z))
     return rc;
+  if (int rc = check_dense(what, weight, y)) return rc;
   const RowView xv{static_cast<const __nv_bfloat16*>(x), x_token_stride, x_head_stride};
   const RowView zv{static_cast<const __nv_bfloat16*>(z), z_token_stride, z_head_stride};
   const unsigned grid = unsigned((rows + kNormRowsPerBlock - 1) / kNormRowsPerBlock);
@@ -370,6 +380,7 @@ int mek_gated_rmsnorm_bwd_kept(const void* dy, const uint8_t* n_codes, const uin
   if (int rc = check_checkpoint("gated_rmsnorm_bwd_kept", kept)) return rc;
   if ((dw == nullptr) != (dw_partial == nullptr))
     return fail(MEK_ERR_INVALID, "gated_rmsnorm_bwd_kept: dw and its partial sums go together");
+  if (int rc = check_dense("gated_rmsnorm_bwd_kept", weight, dy, dx, dz)) return rc;
   if (rows <= 0) return fail(MEK_ERR_INVALID, "gated_rmsnorm_bwd_kept: rows=%lld must be positive", (long long)rows);
   const int blocks = norm_blocks(rows);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -396,6 +407,7 @@ int mek_gated_rmsnorm_bwd(const void* dy, const void* x, const void* z, const vo
   if (int rc = check_norm("gated_rmsnorm_bwd", rows, heads, x_token_stride, x_head_stride, z_token_stride,
                           z_head_stride, x, z))
     return rc;
+  if (int rc = check_dense("gated_rmsnorm_bwd", weight, dy, dx, dz)) return rc;
   const RowView xv{static_cast<const __nv_bfloat16*>(x), x_token_stride, x_head_stride};
   const RowView zv{static_cast<const __nv_bfloat16*>(z), z_token_stride, z_head_stride};
   const int blocks = norm_blocks(rows);
