@@ -79,8 +79,9 @@ def _rows_view(t: torch.Tensor, name: str) -> tuple[torch.Tensor, int, int, int]
         and token_stride >= 0 and head_stride >= 0
     )
     if not in_place:
-        t = t.contiguous()
-        token_stride, head_stride = (t.stride(0), 0) if t.dim() == 2 else (t.stride(0), t.stride(1))
+        t = aligned(t)
+        # not t's own strides: those of an extent of one may be anything in a dense tensor
+        token_stride, head_stride = heads * HEAD_DIM, HEAD_DIM if t.dim() == 3 else 0
     return t, heads, token_stride, head_stride
 
 

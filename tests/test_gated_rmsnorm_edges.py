@@ -92,3 +92,31 @@ def test_the_gradient_of_a_concatenation_of_flat_outputs(checkpoint):
     whole = torch.cat([other, rmsnorm_silu_gate(*leaves, EPS, checkpoint=checkpoint).flatten()])
     got = torch.autograd.grad(whole, leaves, torch.cat([torch.zeros(3, device="cuda", dtype=BF16), dy.flatten()]))
     assert all(torch.equal(a, b) for a, b in zip(got, run(x, z, w, dy, checkpoint)[1:]))
+
+
+def test_rows_that_cannot_be_read_in_place_are_copied():
+    from miles_ext_kernels_b200.cake._impl.gated_rmsnorm.ops import _rows_view
+
+    flat = torch.randn(4000).bfloat16()
+    views = [flat[offset : offset + 3 * 2 * 128].view(3, 2, 128) for offset in (0, 1, 3, 4)]  # dense, at odd addresses
+    views += [v.view(-1, 128) for v in views]
+    views += [flat[: 2 * 1159].view(2, 1159)[:1, 8:136], flat.as_strided((1, 2, 128), (1159, 128, 1), 8),  # one token only
+              flat.as_strided((2, 1, 128), (256, 1159, 1)), flat.as_strided((2, 3, 128), (1159, 128, 1), 1)]
+    for view in views:
+        t, heads, token_stride, head_stride = _rows_view(view, "x")
+        assert heads == (1 if view.dim() == 2 else view.shape[1])
+        assert t.data_ptr() % 16 == 0 and token_stride % 8 == 0 and head_stride % 8 == 0
+        rows = t.as_strided((view.shape[0], heads, 128), (token_stride, head_stride, 1))
+        assert torch.equal(rows.reshape(view.shape), view)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_x_and_z_at_odd_addresses(checkpoint):
+    x, z, w, dy = make(37, 3, seed=2)
+    want = run(x, z, w, dy, checkpoint)
+    for got in (run(moved(x, 1), z, w, dy, checkpoint), run(x, moved(z, 3), w, dy, checkpoint)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    one = torch.randn(2, 1159, device="cuda").bfloat16()[:1, 8:136]  # one row of a projection of odd width
+    got = run(one, one, w, dy[:1, 0], checkpoint)
+    assert all(torch.equal(a, b) for a, b in zip(got, run(one.clone(), one.clone(), w, dy[:1, 0], checkpoint)))
