@@ -2,13 +2,15 @@
 
 An op asks for scratch with :func:`take` under a key ``(op, role)``.  The pool holds at most
 ``--cake-workspace-pool-bytes`` per device.  At the default 0 nothing is held: every ``take`` is a plain
-``torch.empty``.  With a positive bound the pool keeps one byte buffer per ``(op, role)`` and CUDA stream, hands out
-typed views of it while it is large enough, and drops the least recently used buffers to stay under the bound; a
+``torch.empty``.  With a positive bound the pool keeps one byte buffer per ``(op, role)``, CUDA stream and thread, hands
+out typed views of it while it is large enough, and drops the least recently used buffers to stay under the bound; a
 request larger than the bound is served by a plain allocation.  While the current stream captures a CUDA graph the
 pool is bypassed, so a graph never records memory the pool may free later.
 
-A buffer from :func:`take` stays valid until the next :func:`take` of the same key on the same stream, or
-:func:`release`.  Use it on that stream only; never save it for backward and never return it to a caller.
+A buffer from :func:`take` stays valid until the next :func:`take` of the same key on the same stream by the same thread,
+or :func:`release`.  Use it on that stream only; never save it for backward and never return it to a caller.  (Per thread:
+an op enqueues several operations on its scratch, and with one buffer a stream another thread's operations on the same
+stream would come in between.)
 
 Same contract as the reference's pool (reference: miles_ext_kernels/cake/_runtime/workspace.py:77-141).  Importing
 this module does not import torch.
@@ -31,7 +33,7 @@ class _DevicePool:
     """The buffers of one device, least recently used first, and its counters."""
 
     def __init__(self) -> None:
-        self.buffers: OrderedDict[tuple[str, str, Any], Any] = OrderedDict()
+        self.buffers: OrderedDict[tuple[str, str, Any, int], Any] = OrderedDict()
         self.hits = self.misses = self.evictions = 0
 
     def held(self) -> int:
@@ -76,7 +78,7 @@ def _current_stream(key: Any) -> tuple[Any, bool]:
 
 def take(op: str, role: str, shape: Sequence[int], dtype: Any, device: Any) -> Any:
     """A tensor of ``shape`` / ``dtype`` on ``device`` with undefined content: a view of the pooled buffer of
-    ``(op, role)`` on the current stream, or a plain ``torch.empty`` when the pool does not serve the request."""
+    ``(op, role)`` of the current stream and thread, or a plain ``torch.empty`` when the pool does not serve the request."""
     import torch
 
     bound = config.pool_bytes()
@@ -96,7 +98,7 @@ def take(op: str, role: str, shape: Sequence[int], dtype: Any, device: Any) -> A
         return torch.empty(shape, dtype=dtype, device=where)
 
     nbytes = math.prod(shape) * dtype.itemsize
-    slot = (op, role, stream)
+    slot = (op, role, stream, threading.get_ident())
     with _lock:
         buffer = pool.buffers.get(slot)
         if buffer is not None and nbytes <= buffer.numel() <= bound:
@@ -119,7 +121,7 @@ def take(op: str, role: str, shape: Sequence[int], dtype: Any, device: Any) -> A
 
 
 def release(op: str | None = None) -> int:
-    """Drop the pooled buffers of every op, or of ``op``, on every device and stream; returns the bytes dropped."""
+    """Drop the pooled buffers of every op, or of ``op``, of every device, stream and thread; returns the bytes dropped."""
     freed = 0
     with _lock:
         for pool in _pools.values():

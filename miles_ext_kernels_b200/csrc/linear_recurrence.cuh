@@ -173,6 +173,8 @@ struct GlrShared {
 };
 
 // The block's tile -- the next in order, or its own index where tiles do not wait for one another -- and the barriers.
+// tile < 0: a number behind the last tile, which only a counter that something else writes to can give; the block has
+// nothing to do.
 template <bool kReverse, int kDirections>
 __device__ __forceinline__ GlrTileAt take_tile(const GlrShape& s, GlrShared<kDirections>& sh) {
   if (threadIdx.x < 32) {
@@ -181,6 +183,7 @@ __device__ __forceinline__ GlrTileAt take_tile(const GlrShape& s, GlrShared<kDir
     if (threadIdx.x == 0) {
       const int index = s.counter ? atomicAdd(s.counter, 1) + 1 : int(blockIdx.x);
       sh.at = tile_at<kReverse>(s, index);
+      if (unsigned(index) >= gridDim.x) sh.at.tile = -1;
       sh.ahead = tile_at<kReverse>(s, min(index, int(gridDim.x) - 1 - s.ahead) + s.ahead);
       if (index >= int(gridDim.x) - s.ahead) sh.ahead.tile = -1;
       sh.late = 0;

@@ -22,6 +22,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   __shared__ GlrShared<2> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const GlrTileAt at = take_tile<true>(s, sh);
+  if (at.tile < 0) return;
   const int t0 = at.tile * kGlrTile + warp * kGlrTokens;
   float* decay = reinterpret_cast<float*>(smem + warp * kGlrDecays);
   X* xs = reinterpret_cast<X*>(smem + kGlrWarps * kGlrDecays + warp * kGlrBox<X>);

@@ -18,6 +18,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   __shared__ GlrShared<1> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const GlrTileAt at = take_tile<false>(s, sh);
+  if (at.tile < 0) return;
   const int t0 = at.tile * kGlrTile + warp * kGlrTokens;
   float* decay = reinterpret_cast<float*>(smem + warp * kGlrDecays);
   X* xs = reinterpret_cast<X*>(smem + kGlrWarps * kGlrDecays + warp * kGlrBox<X>);
