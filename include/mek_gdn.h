@@ -74,6 +74,13 @@ int mek_selftest_tma(const void* src, int64_t rows, int64_t cols, int box_rows, 
 int mek_selftest_umma_rate(int m, int n, int a_mn, int b_mn, int kdim, int count, int issuers, int interleave,
                            long long* cycles, int32_t* status, void* stream);
 
+/* Waits of the row operators' launches that follow in this process (LayerNorm, the linear recurrence), for the tests of a
+ * wait that runs out: limit_ns, at most and as a rule one second (negative: that), and what is not sent -- LayerNorm's
+ * streamed rows from rows_served on (negative: all are sent), and by bit of tiles_withheld, of every tile of the
+ * recurrence, the tokens of warp 0..7 (where they come by TMA) or, bit 8, the words that carry the state to other
+ * tiles.  What is withheld is never asked for, so nothing is in flight when a block ends. */
+int mek_selftest_row_waits(int64_t limit_ns, int64_t rows_served, uint32_t tiles_withheld);
+
 /* Extents and chunk tables of one call.  Tokens are packed: [total_tokens, heads, 128]; a batch of B equal-length
  * sequences is B sequences of one packed row.  Chunks hold at most 64 tokens and never straddle a sequence.
  * Replaces the reference's ChunkMeta int32 tables (reference: miles_ext_kernels/cake/_impl/gdn/ops.py:157-174). */

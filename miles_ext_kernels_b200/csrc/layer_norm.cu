@@ -228,7 +228,7 @@ template <typename T, int VEC, int G, int NV>
 __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlocks<G>) layer_norm_fwd_kernel(
     const T* __restrict__ x, int64_t x_stride, const void* __restrict__ weight, const void* __restrict__ bias,
     int param_type, T* __restrict__ y, float* __restrict__ mean_out, float* __restrict__ rstd_out,
-    uint8_t* __restrict__ codes, int64_t rows, int width, float eps, int slots) {
+    uint8_t* __restrict__ codes, int64_t rows, int width, float eps, int slots, const RowWaits waits) {
   typedef RowShape<T, VEC, G, NV> Shape;
   constexpr bool kStream = kLnStreams<VEC, G>;
   constexpr int kPairs = Shape::kPairs;
@@ -239,10 +239,11 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
   const int lane = threadIdx.x % G, warp = lane / 32;
   const uint32_t bytes = uint32_t(width) * sizeof(T);
   const int64_t first = int64_t(blockIdx.x) * Shape::kRows + threadIdx.x / G, step = int64_t(gridDim.x) * Shape::kRows;
+  const int64_t served = rows < waits.rows_served ? rows : waits.rows_served;
   if (kStream && threadIdx.x == 0) {
     for (int k = 0; k < slots; ++k) mbar_init(&s_full[k], 1);
     fence_mbar_init();
-    for (int k = 0; k < slots && first + k * step < rows; ++k) {
+    for (int k = 0; k < slots && first + k * step < served; ++k) {
       mbar_arrive_expect(&s_full[k], bytes);
       bulk_load(smem + k * bytes, x + (first + k * step) * x_stride, bytes, &s_full[k]);
     }
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
   auto one_row = [&](int64_t r, RowPart<T, VEC, G, NV>& part) {
     const bool live = Shape::kSide == 1 || r < rows;  // rows side by side in a warp go through its shuffles together
     if constexpr (kStream) {
-      if (!failed) failed = !mbar_wait_soon(&s_full[slot], parity);
+      if (!failed) failed = !mbar_wait_soon(&s_full[slot], parity, waits.limit_ns);
       part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
     }
     Two xv[kPairs], sum = two(0.f);
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnFwdBlock
     if constexpr (G > 32) {  // the warps' by Chan's rule
       if (threadIdx.x % 32 == 0) s_part[phase][warp] = make_float2(mean, m2);
       __syncthreads();
-      if (kStream && threadIdx.x == 0 && !failed && r + slots * step < rows) {  // everybody has the row in registers
+      if (kStream && threadIdx.x == 0 && !failed && r + slots * step < served) {  // everybody has the row in registers
         mbar_arrive_expect(&s_full[slot], bytes);
         bulk_load(smem + slot * bytes, x + (r + slots * step) * x_stride, bytes, &s_full[slot]);
       }
@@ -358,7 +359,8 @@ template <typename T, int VEC, int G, int NV, bool kCodes, bool kStream>
 __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlocks<G>) layer_norm_bwd_kernel(
     const T* __restrict__ dy, const T* __restrict__ x, int64_t x_stride, const uint8_t* __restrict__ codes,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, const void* __restrict__ weight,
-    int param_type, T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width, int slots) {
+    int param_type, T* __restrict__ dx, float* __restrict__ partial, int64_t rows, int width, int slots,
+    const RowWaits waits) {
   typedef RowShape<T, VEC, G, NV> Shape;
   typedef typename std::conditional<kCodes, uint8_t, T>::type Kept;
   constexpr int kPairs = Shape::kPairs;
@@ -369,6 +371,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
   const uint32_t dy_bytes = uint32_t(width) * sizeof(T), kept_bytes = uint32_t(width) * sizeof(Kept);
   const uint32_t bytes = dy_bytes + kept_bytes;
   const int64_t first = int64_t(blockIdx.x) * Shape::kRows + threadIdx.x / G, step = int64_t(gridDim.x) * Shape::kRows;
+  const int64_t served = rows < waits.rows_served ? rows : waits.rows_served;
   auto kept_row = [&](int64_t r) -> const Kept* {
     if constexpr (kCodes) return codes + r * width;
     else return x + r * x_stride;
@@ -382,7 +385,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
   if (kStream && threadIdx.x == 0) {
     for (int k = 0; k < slots; ++k) mbar_init(&s_full[k], 1);
     fence_mbar_init();
-    for (int k = 0; k < slots && first + k * step < rows; ++k) fill(k, first + k * step);
+    for (int k = 0; k < slots && first + k * step < served; ++k) fill(k, first + k * step);
   }
   RowParams<T, VEC, G, NV> w;
   w.load(weight, param_type, 1.f, reinterpret_cast<float*>(smem + size_t(kStream ? slots : 0) * bytes), lane, width);
@@ -416,7 +419,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
     RowPart<T, VEC, G, NV> g_part;
     RowPart<Kept, VEC, G, NV> k_part;
     if constexpr (kStream) {
-      if (!failed) failed = !mbar_wait_soon(&s_full[slot], parity);
+      if (!failed) failed = !mbar_wait_soon(&s_full[slot], parity, waits.limit_ns);
       g_part.load(reinterpret_cast<const T*>(smem + slot * bytes), lane, width);
       k_part.load(reinterpret_cast<const Kept*>(smem + slot * bytes + dy_bytes), lane, width);
     } else {
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
     }
     const float2 a = split(s1), c = split(s2);
     const float2 sums = group_sum<G>(failed ? __int_as_float(0x7fffffff) : a.x + a.y, c.x + c.y, s_part, phase);
-    if (kStream && threadIdx.x == 0 && !failed && r + slots * step < rows) fill(slot, r + slots * step);  // all have read the row
+    if (kStream && threadIdx.x == 0 && !failed && r + slots * step < served) fill(slot, r + slots * step);  // all have read the row
     const Two m1 = two(sums.x * inv_width), m2 = two(-(sums.y * inv_width));
     if (live) store_row<T, VEC, G, NV>(dx + r * width, lane, width, [&](int q) {
       return mul2(fma2(unit(q), m2, sub2(mul2(g_part.pair(q), w.pair(q, lane)), m1)), scale);
@@ -650,7 +653,8 @@ int ln_fwd(const LnPlan& p, const void* x, int64_t xs, const void* w, const void
   if (smem > 40 << 10)  // with the static part it may pass the 48 KB a launch has without asking
     if (int rc = want_smem(layer_norm_fwd_kernel<T, VEC, G, NV>, smem, "layer_norm_fwd")) return rc;
   layer_norm_fwd_kernel<T, VEC, G, NV><<<p.grid, RowShape<T, VEC, G, NV>::kThreads, smem, s>>>(
-      static_cast<const T*>(x), xs, w, b, pt, static_cast<T*>(y), mean, rstd, codes, rows, width, eps, p.slots);
+      static_cast<const T*>(x), xs, w, b, pt, static_cast<T*>(y), mean, rstd, codes, rows, width, eps, p.slots,
+      row_waits());
   return launched("layer_norm_fwd");
 }
 template <typename T, int VEC, int G, int NV, bool kCodes, bool kStream>
@@ -662,7 +666,7 @@ int ln_bwd_of(const LnPlan& p, const void* dy, const void* x, int64_t xs, const 
     if (int rc = want_smem(layer_norm_bwd_kernel<T, VEC, G, NV, kCodes, kStream>, smem, "layer_norm_bwd")) return rc;
   layer_norm_bwd_kernel<T, VEC, G, NV, kCodes, kStream><<<p.grid, RowShape<T, VEC, G, NV>::kThreads, smem, s>>>(
       static_cast<const T*>(dy), static_cast<const T*>(x), xs, codes, mean, rstd, w, pt, static_cast<T*>(dx), partial, rows,
-      width, p.slots);
+      width, p.slots, row_waits());
   return launched("layer_norm_bwd");
 }
 template <typename T, int VEC, int G, int NV>

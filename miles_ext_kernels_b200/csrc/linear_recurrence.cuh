@@ -149,6 +149,7 @@ struct GlrShape {
   int window;        // words a warp looks back over at once; 0: one warp looks at the nearest four
   int ahead;         // how many tiles later lies the one a block asks into L2
   int* counter;      // the last tile taken (-1 before the launch); NULL where there is one tile a chain
+  RowWaits waits;
 };
 struct GlrTileAt {
   int b, tile, c0;
@@ -304,6 +305,7 @@ __device__ __forceinline__ Words load_words(const float* row, const GlrShape& s,
 }
 template <bool kPair>
 __device__ __forceinline__ void publish(float* row, const GlrShape& s, const GlrTileAt& at, const Words& v) {
+  if (s.waits.tiles_withheld & kWithholdWords) return;
   const int left = s.channels - at.c0 - 2 * int(threadIdx.x & 31);
   const Two w[2] = {two(v.A0, v.B0), two(v.A1, v.B1)};
   if constexpr (kPair) {
@@ -346,7 +348,8 @@ __device__ __forceinline__ Two look_back(float* words, const GlrShape& s, const 
     if (polls >= kGlrFreePolls) {  // reading the timer costs as much as a poll: the first ones go without
       const uint64_t now = global_timer_ns();
       if (began == 0) began = now;
-      if (now - began > kWaitLimitNs) return two(__int_as_float(0x7fffffff));
+      // one decision for the warp: a lane that left alone would be waited for in the votes above
+      if (__any_sync(0xffffffffu, now - began > s.waits.limit_ns)) return two(__int_as_float(0x7fffffff));
     }
   }
 }
@@ -384,7 +387,7 @@ __device__ __forceinline__ void look_back_together(float* words, const GlrShape&
     if (threadIdx.x == 0 && polls >= kGlrFreePolls) {
       const uint64_t now = global_timer_ns();
       if (began == 0) began = now;
-      if (now - began > kWaitLimitNs) sh.late = 1;
+      if (now - began > s.waits.limit_ns) sh.late = 1;
     }
     __syncthreads();
     const int2 mark = sh.marks[lane & (kGlrWarps - 1)];
@@ -566,7 +569,7 @@ inline int size_of(int type) { return type == kTypeFp32 ? 4 : 2; }
 
 inline GlrShape glr_shape(int64_t batch, int64_t tokens, int64_t channels, int64_t seqs, const int32_t* cu) {
   return {{cu, int(cu ? seqs : batch), int(tokens)}, int(batch), int(tokens), int(channels),
-          int((tokens + kGlrTile - 1) / kGlrTile), int((channels + kGlrChannels - 1) / kGlrChannels), 0, 0, nullptr};
+          int((tokens + kGlrTile - 1) / kGlrTile), int((channels + kGlrChannels - 1) / kGlrChannels), 0, 0, nullptr, row_waits()};
 }
 
 // The window: words a warp looks back over, eight warps together.  With few chains (channel blocks x batch rows) the tiles

@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   bool arrived = true;
   const bool any = t0 < s.tokens;  // a warp behind the last token only takes part in the block's barriers
   if constexpr (kTma) {
-    if (lane == 0 && any) {
+    if (lane == 0 && any && !((s.waits.tiles_withheld >> warp) & 1)) {
       mbar_arrive_expect(&sh.arrived[warp], 2 * kGlrBox<X> + kGlrBox<G>);
       box_load(gs, &g_map, at.c0, t0, at.b, &sh.arrived[warp]);
       box_load(ds, &dy_map, at.c0, t0, at.b, &sh.arrived[warp]);
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   const Edges edges = any ? Edges(s.seq, span_of(s.seq, t0), at.b, t0) : Edges();
   const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
   const Two d1 = edges.end >= 0 ? load_state<kTma>(p.d_final, s, at, edges.end_seq) : two(0.f);
-  if (kTma && any) arrived = mbar_wait_soon(&sh.arrived[warp], 0);
+  if (kTma && any) arrived = mbar_wait_soon(&sh.arrived[warp], 0, s.waits.limit_ns);
   {
     Two A = two(1.f), B = two(0.f), D = two(0.f);
     if (any) {

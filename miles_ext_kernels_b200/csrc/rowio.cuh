@@ -153,12 +153,26 @@ __device__ __forceinline__ float code_value(uint8_t code) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3)));
 }
 
-// mbar_wait for copies that are on their way as a rule: the first looks go without the timer, whose reading costs more than
+// How long the row operators' kernels wait, and, for the tests of a wait that runs out, what is not sent
+// (mek_selftest_row_waits; as a rule one second, and everything is).
+struct RowWaits {
+  uint32_t limit_ns;
+  uint32_t tiles_withheld;  // linear recurrence: bit w: the tokens of warp w of each tile; kWithholdWords: the tiles' words
+  int64_t rows_served;      // LayerNorm: rows from here on are not copied where rows are streamed
+};
+constexpr uint32_t kWithholdWords = 1u << 8;
+RowWaits row_waits();  // what the next launch takes
+
+// A wait for copies that are on their way as a rule: the first looks go without the timer, whose reading costs more than
 // a look (and is shared by the SM).
-__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, uint32_t limit_ns) {
   for (int looks = 0; looks < 256; ++looks)
     if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait(bar, parity);
+  const uint64_t began = global_timer_ns();
+  for (;;) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (global_timer_ns() - began > limit_ns) return false;
+  }
 }
 
 // After a wait that ran out: copies that are still in flight may write to this block's shared memory.

@@ -1,5 +1,8 @@
 // Self-test of the tcgen05 building block and the library-wide C-ABI helpers (version stamp, error text, device gate).
+#include <atomic>
+
 #include "common.cuh"
+#include "rowio.cuh"
 #include "tma.cuh"
 #include "umma.cuh"
 
@@ -9,6 +12,10 @@ char* error_buffer() {
   static thread_local char text[512] = {0};
   return text;
 }
+
+static std::atomic<int64_t> wait_limit_ns{int64_t(kWaitLimitNs)}, wait_rows_served{INT64_MAX};
+static std::atomic<uint32_t> wait_tiles_withheld{0};
+RowWaits row_waits() { return {uint32_t(wait_limit_ns.load()), wait_tiles_withheld.load(), wait_rows_served.load()}; }
 
 // Operand images are copied verbatim into shared memory; the caller's descriptors decide how the tensor core reads
 // them.  128 threads: thread t dumps tensor-memory lane t.
@@ -157,6 +164,15 @@ __global__ void __launch_bounds__(128) umma_rate_kernel(int a_mn, int b_mn, int 
 extern "C" {
 
 int mek_build_cuda_version(void) { return CUDART_VERSION; }
+
+int mek_selftest_row_waits(int64_t limit_ns, int64_t rows_served, uint32_t tiles_withheld) {
+  using namespace mek;
+  if (limit_ns > int64_t(kWaitLimitNs)) return fail(MEK_ERR_INVALID, "selftest_row_waits: a wait lasts at most one second");
+  wait_limit_ns = limit_ns < 0 ? int64_t(kWaitLimitNs) : limit_ns;
+  wait_rows_served = rows_served < 0 ? INT64_MAX : rows_served;
+  wait_tiles_withheld = tiles_withheld;
+  return MEK_OK;
+}
 
 const char* mek_last_error(void) { return mek::error_buffer(); }
 
