@@ -277,6 +277,7 @@ __device__ __forceinline__ void store_state(float* __restrict__ state, const Glr
 }
 
 // ---- the words between tiles: (A, B) per tile and channel, all ones before the launch --------------------------------
+__device__ __forceinline__ Two lost() { return two(__int_as_float(0x7fffffff)); }  // a state that did not come in time: NaN
 struct Words {  // of a lane's two channels
   float A0, B0, A1, B1;
   __device__ __forceinline__ bool set() const {
@@ -349,7 +350,7 @@ __device__ __forceinline__ Two look_back(float* words, const GlrShape& s, const 
       const uint64_t now = global_timer_ns();
       if (began == 0) began = now;
       // one decision for the warp: a lane that left alone would be waited for in the votes above
-      if (__any_sync(0xffffffffu, now - began > s.waits.limit_ns)) return two(__int_as_float(0x7fffffff));
+      if (__any_sync(0xffffffffu, now - began > s.waits.limit_ns)) return lost();
     }
   }
 }
@@ -394,7 +395,7 @@ __device__ __forceinline__ void look_back_together(float* words, const GlrShape&
     unset = __reduce_min_sync(0xffffffffu, mark.x), from = __reduce_min_sync(0xffffffffu, mark.y);
     if (from < unset) break;
     if (sh.late != 0) {
-      sh.carried[lane] = two(__int_as_float(0x7fffffff));  // every warp the same
+      sh.carried[lane] = lost();  // every warp the same
       __syncthreads();
       return;
     }

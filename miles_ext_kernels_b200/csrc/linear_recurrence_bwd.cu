@@ -56,9 +56,10 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
     h = two(v.B0, v.B1);
   }
   const Edges edges = any ? Edges(s.seq, span_of(s.seq, t0), at.b, t0) : Edges();
-  const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
-  const Two d1 = edges.end >= 0 ? load_state<kTma>(p.d_final, s, at, edges.end_seq) : two(0.f);
-  if (kTma && any) arrived = mbar_wait_soon(&sh.arrived[warp], 0, s.waits.limit_ns);
+  Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
+  Two d1 = edges.end >= 0 ? load_state<kTma>(p.d_final, s, at, edges.end_seq) : two(0.f);
+  if (kTma && any) arrived = __all_sync(0xffffffffu, mbar_wait_soon(&sh.arrived[warp], 0, s.waits.limit_ns));
+  if (!arrived) s0 = d1 = lost();  // whatever lies in the tile, every gradient of the warp and what it hands on is NaN
   {
     Two A = two(1.f), B = two(0.f), D = two(0.f);
     if (any) {
@@ -72,7 +73,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
     }
     if (edges.starts) A = two(kGlrReset);
     if (edges.ends) R = two(kGlrReset);
-    if (!arrived) R = two(kGlrReset), D = two(__int_as_float(0x7fffffff));
+    if (!arrived) A = R = two(kGlrReset), B = D = lost();
     sh.pair[0][warp][lane] = packed(A, B);
     sh.pair[1][warp][lane] = packed(R, D);
   }
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
 #pragma unroll
   for (int w = kGlrWarps - 1; w > 0; --w)
     if (w > warp) c = folded(sh.pair[1][w][lane], c);
-  if (!arrived) c = two(__int_as_float(0x7fffffff));
+  if (!arrived) h = c = lost();
   if (!any) return;
   // forward once more for the state before every token, then back with the adjoint; dx takes dy's place, dg the gates'
   Two before[kGlrTokens];
@@ -112,13 +113,15 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
 #pragma unroll
     for (int j = 0; j < kGlrTokens; ++j) {
       if (j == edges.start) h = s0;
-      if (!one && ((edges.starts >> j) & 1)) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t0 + j));
+      if (!one && ((edges.starts >> j) & 1))
+        h = arrived ? load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t0 + j)) : lost();
       before[j] = h, h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
     }
 #pragma unroll
     for (int j = kGlrTokens - 1; j >= 0; --j) {
       if (j == edges.end) c = d1;
-      if (!one && ((edges.ends >> j) & 1)) c = load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t0 + j));
+      if (!one && ((edges.ends >> j) & 1))
+        c = arrived ? load_state<kTma>(p.d_final, s, at, sequence_of(s.seq, at.b, t0 + j)) : lost();
       const Two dh = add2(widened(token(ds, j)), c);
       c = mul2(decay_at(decay, j), dh);
       const bool live = (edges.live >> j) & 1;

@@ -41,8 +41,9 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
     __syncwarp();
   }
   const Edges edges = any ? Edges(s.seq, span_of(s.seq, t0), at.b, t0) : Edges();
-  const Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
-  if (kTma && any) arrived = mbar_wait_soon(&sh.arrived[warp], 0, s.waits.limit_ns);
+  Two s0 = edges.start >= 0 ? load_state<kTma>(p.h0, s, at, edges.start_seq) : two(0.f);
+  if (kTma && any) arrived = __all_sync(0xffffffffu, mbar_wait_soon(&sh.arrived[warp], 0, s.waits.limit_ns));
+  if (!arrived) s0 = lost();  // whatever lies in the tile, from here on every token and state of the warp is NaN
   const Two none = two(0.f);
   Two A = two(1.f), B = none, no_adjoint;
   if (any) {
@@ -51,7 +52,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
   }
   if (edges.kind == kManyEdges) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
   if (edges.starts) A = two(kGlrReset);
-  if (!arrived) A = two(kGlrReset), B = two(__int_as_float(0x7fffffff));
+  if (!arrived) A = two(kGlrReset), B = lost();
   sh.pair[0][warp][lane] = packed(A, B);
   __syncthreads();
   Two h = two(0.f);
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
 #pragma unroll
   for (int w = 0; w < kGlrWarps - 1; ++w)
     if (w < warp) h = folded(sh.pair[0][w][lane], h);
-  if (!arrived) h = two(__int_as_float(0x7fffffff));
+  if (!arrived) h = lost();
   if (!any) return;
   if (edges.kind == kInside) {
 #pragma unroll
@@ -89,7 +90,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
 #pragma unroll 1
     for (int j = 0; j < kGlrTokens; ++j) {
       const int t = t0 + j;
-      if ((edges.starts >> j) & 1) h = load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t));
+      if ((edges.starts >> j) & 1) h = arrived ? load_state<kTma>(p.h0, s, at, sequence_of(s.seq, at.b, t)) : lost();
       h = fma2(decay_at(decay, j), h, widened(token(xs, j)));
       const bool live = (edges.live >> j) & 1;
       token(xs, j) = narrowed<X>(live ? h : two(0.f));

@@ -81,3 +81,58 @@ def test_words_that_do_not_come(channels):
     assert got["dh0"].isnan().all() and torch.equal(got["y"], want["y"])
     again = recurrence(x, g, h0, dy, dl, cuts)
     assert all(torch.equal(again[n], want[n]) for n in want)
+
+
+LAYOUTS = {
+    "one": [3 * TILE + 70],
+    "two in a warp": [TILE + 53, 200],  # starts and ends inside the warp that is kept back
+    "many in a warp": [TILE + 50, 3, 1, 4, 0, 130, 20],
+    "at its borders": [48, 16, 64, 48, 100],
+    "short": [5] * 40,
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gdtype", [FP32, BF16])
+@pytest.mark.parametrize("layout", LAYOUTS)
+def test_tokens_that_do_not_come(layout, gdtype):
+    """One warp's tokens of every tile: NaN, like all that follows from them inside their sequence."""
+    warp, channels, lengths = 3, 128, LAYOUTS[layout]
+    tokens = sum(lengths)
+    x, g, dy = sequence(tokens, channels, seed=1)
+    g = g.to(gdtype)
+    cuts = torch.tensor([0] + lengths, device="cuda").cumsum(0).int()
+    n = len(lengths)
+    h0, dl = torch.randn(n, channels, device="cuda"), torch.randn(n, channels, device="cuda")
+    want = recurrence(x, g, h0, dy, dl, cuts)
+    kept_back = lambda t: t % TILE // WARP == warp  # noqa: E731
+    spans = [(sum(lengths[:i]), sum(lengths[: i + 1])) for i in range(n)]
+    state, adjoint, before = [False] * tokens, [False] * tokens, [False] * tokens
+    for lo, hi in spans:
+        bad = inside = False
+        for t in range(lo, hi):
+            inside = inside and t % TILE != 0  # the backward starts each tile from the forward's state
+            before[t] = inside or kept_back(t)
+            bad, inside = bad or kept_back(t), inside or kept_back(t)
+            state[t] = bad
+        bad = False
+        for t in reversed(range(lo, hi)):
+            bad = bad or kept_back(t)
+            adjoint[t] = bad
+    assert any(state) and any(adjoint)
+
+    def check(got, n, lost):
+        lost = torch.tensor(lost, device="cuda")
+        where = lost[None, :, None] if got[n].dim() == 3 else lost[:, None]
+        assert torch.equal(got[n].isnan(), where.expand_as(got[n])), n
+        assert torch.equal(torch.where(where, 0, got[n]), torch.where(where, 0, want[n])), n
+
+    got = recurrence(x, g, h0, dy, dl, cuts, forward=dict(tiles=1 << warp))
+    check(got, "y", state)
+    check(got, "final", [hi > lo and state[hi - 1] for lo, hi in spans])
+    got = recurrence(x, g, h0, dy, dl, cuts, backward=dict(tiles=1 << warp))
+    check(got, "dx", adjoint)
+    check(got, "dg", [a or b for a, b in zip(adjoint, before)])
+    check(got, "dh0", [hi > lo and adjoint[lo] for lo, hi in spans])
+    again = recurrence(x, g, h0, dy, dl, cuts)
+    assert all(torch.equal(again[n], want[n]) for n in want)
