@@ -9,7 +9,9 @@
  *     ValueError, MEK_ERR_CUDA -> RuntimeError, as the reference's typed tvm-ffi exceptions do
  *     (reference: tools/templates/cake_host_shim.h:52-114);
  *   - kernels with bounded waits write a nonzero word to `status` (device int32) instead of hanging; the caller
- *     reads it after synchronising the stream.
+ *     reads it after synchronising the stream.  LayerNorm and the linear recurrence take no such word: what a wait that
+ *     ran out leaves unknown comes out as NaN -- the rows or tokens, all that follows from them inside their sequence, the
+ *     final and initial states' values, the parameters' gradients.
  *
  * The reference exports, per generated library, a tvm-ffi typed function run(tensors..., scalars..., grid_x, grid_y,
  * grid_z) and build_cuda_version() (reference: tools/templates/cake_host_shim.h:62-64).  The entry points below

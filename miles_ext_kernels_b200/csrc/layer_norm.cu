@@ -457,7 +457,11 @@ __global__ void __launch_bounds__(RowShape<T, VEC, G, NV>::kThreads, kLnBwdBlock
     for (int k = 0; k < kDepth; ++k)
       if (r - side + k * step < rows) one_row(r + k * step, k);
   }
-  if (kStream && failed) let_copies_land();
+  if (kStream && failed) {
+    let_copies_land();
+#pragma unroll
+    for (int q = 0; q < kPairs; ++q) dw[q] = db[q] = two(__int_as_float(0x7fffffff));  // they hold whatever lay in the slots
+  }
   if (partial == nullptr) return;
   float* mine = partial + int64_t(blockIdx.x) * 2 * width;
   if constexpr (Shape::kRows == 1) {

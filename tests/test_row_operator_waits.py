@@ -136,3 +136,33 @@ def test_tokens_that_do_not_come(layout, gdtype):
     check(got, "dh0", [hi > lo and adjoint[lo] for lo, hi in spans])
     again = recurrence(x, g, h0, dy, dl, cuts)
     assert all(torch.equal(again[n], want[n]) for n in want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+@pytest.mark.parametrize("width,dtype", [(1024, BF16), (4096, BF16), (16384, BF16), (2048, FP32), (8192, FP32)])
+def test_rows_that_do_not_come(width, dtype, checkpoint):
+    """Streamed rows from one row on: their outputs are NaN, and so are the parameters' gradients, which need every row."""
+    from miles_ext_kernels_b200.cake.layer_norm import layer_norm
+
+    rows, served = 1500, 700
+    gen = torch.Generator(device="cuda").manual_seed(width)
+    randn = lambda *s: torch.randn(*s, device="cuda", generator=gen).to(dtype)  # noqa: E731
+    x, w, b, dy = randn(rows, width), randn(width), randn(width), randn(rows, width)
+
+    def step(forward=None, backward=None):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        with withheld(**(forward or {})):
+            y = layer_norm(*leaves, checkpoint=checkpoint)
+        with withheld(**(backward or {})):
+            return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = step()
+    y, dx, dw, _ = step(forward=dict(rows_served=served))
+    for got, ref in ((y, want[0]), (dx, want[1])):  # the statistics and the codes of those rows are NaN as well
+        assert torch.equal(got[:served], ref[:served]) and got[served:].isnan().all()
+    assert dw.isnan().all()
+    y, dx, dw, db = step(backward=dict(rows_served=served))
+    assert torch.equal(y, want[0]) and torch.equal(dx[:served], want[1][:served]) and dx[served:].isnan().all()
+    assert dw.isnan().all() and db.isnan().all()
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
