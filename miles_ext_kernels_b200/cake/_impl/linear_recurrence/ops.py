@@ -16,6 +16,7 @@ from pathlib import Path
 from typing import Any
 
 import torch
+from torch.autograd.graph import increment_version
 
 from ..._runtime import loader, registry, workspace
 from ..gdn import native
@@ -235,9 +236,10 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
 
     ``x``: BF16, FP16 or FP32 ``[R, ...]``; ``g``: the log decay in nats, ``x``'s shape, in any of the three types.
     ``state``: the FP32 pool ``[N, ...]``, dense inside a slot (any stride between them), updated in place, so not for
-    autograd.  ``state_indices``: int32 or int64 ``[R]``, the slot of every row (``None``: row ``r`` uses slot ``r`` and
-    ``N >= R``).  A row whose index is outside ``[0, N)``, -1 for example, is padding: no state changes and its ``y`` is
-    zero.  Rows that name one slot are applied one after the other, in row order."""
+    autograd (a recorded call that saved the pool, as its ``initial_state`` for example, raises in its backward).
+    ``state_indices``: int32 or int64 ``[R]``, the slot of every row (``None``: row ``r`` uses slot ``r`` and ``N >= R``).
+    A row whose index is outside ``[0, N)``, -1 for example, is padding: no state changes and its ``y`` is zero.  Rows that
+    name one slot are applied one after the other, in row order."""
     device, shape, trailing = x.device, x.shape, state.shape[1:]
     if not (  # one test for the usual call; _explain_step says what is wrong with any other
         x.is_cuda and x.dim() == 2 and g.shape == shape and trailing == shape[1:] and state.dtype is torch.float32
@@ -267,6 +269,8 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
         _step(device, xv.data_ptr(), TYPES[x.dtype], gv.data_ptr(), TYPES[g.dtype], pooled.data_ptr(), pointer(slots),
               slots is not None and slots.dtype == torch.int64, y.data_ptr(), rows, pool, channels, xv.stride(0),
               gv.stride(0), pooled.stride(0))
+    if not state.is_inference():  # a graph that saved the pool as it was has to hear of the change
+        increment_version(state)
     return y
 
 
