@@ -23,7 +23,7 @@ import torch
 from ..._runtime import config, loader, registry, workspace
 from ..gdn import native
 from ..gdn.native import pointer
-from ..rows import aligned, checkpoint_format, on_device
+from ..rows import aligned, checkpoint_format, on_device, recorded
 
 __all__ = ["check_supported", "prebuild", "release", "rmsnorm_silu_gate"]
 
@@ -100,6 +100,7 @@ class _RmsnormSiluGate(torch.autograd.Function):
         y = torch.empty_like(x, memory_format=torch.contiguous_format)
         rows = x.numel() // HEAD_DIM
         kept = ()
+        keep = keep and any(ctx.needs_input_grad)
         if keep:
             kept = (x.new_empty((rows, HEAD_DIM), dtype=torch.uint8), x.new_empty((rows, HEAD_DIM), dtype=torch.uint8),
                     x.new_empty(rows, dtype=torch.uint8), x.new_empty(rows, dtype=torch.float32))
@@ -161,8 +162,7 @@ def rmsnorm_silu_gate(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, ep
     the gradients).  ``y`` does not
     change."""
     config.variant(OP)  # both variants run the same kernels; an unknown configuration still raises here
-    keep = checkpoint_format(OP, checkpoint) and torch.is_grad_enabled() and (
-        x.requires_grad or z.requires_grad or weight.requires_grad)
+    keep = checkpoint_format(OP, checkpoint) and (torch.is_grad_enabled() or recorded())
     return _RmsnormSiluGate.apply(x, z, weight, eps, keep)
 
 

@@ -26,7 +26,7 @@ import torch
 from ..._runtime import loader, registry, workspace
 from ..gdn import native
 from ..gdn.native import pointer
-from ..rows import TYPES, check_device, checkpoint_format, on_device, once_differentiable
+from ..rows import TYPES, check_device, checkpoint_format, on_device, once_differentiable, recorded
 
 __all__ = ["check_supported", "layer_norm", "prebuild", "release"]
 
@@ -131,9 +131,10 @@ def _gradients(ctx, dy):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
-        y, kept = _forward(x, weight, bias, eps, keep, True)
-        ctx.save_for_backward(*kept, weight, bias)
-        ctx.shape = x.shape
+        y, kept = _forward(x, weight, bias, eps, keep, any(ctx.needs_input_grad))
+        if kept is not None:
+            ctx.save_for_backward(*kept, weight, bias)
+            ctx.shape = x.shape
         return y
 
     backward = staticmethod(once_differentiable(_gradients))
@@ -167,7 +168,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``x``: BF16, FP16 or FP32 on a B200, read in place when its rows have unit stride inside and one stride between
     them, else copied once.  ``weight``, ``bias``: ``[C]``, each optional, both of one type out of the three, which their
     gradients have too.  ``checkpoint``: ``None`` keeps ``x`` for the backward, ``"e4m3"`` keeps the normalised rows in 8
-    bits instead (``C`` up to 200,704).  Not twice differentiable."""
+    bits instead (``C`` up to 200,704).  Not twice differentiable, and
+    without a forward-mode derivative."""
     keep = checkpoint is not None and checkpoint_format(OP, checkpoint)
     if not (  # one test for the usual call; _explain says what is wrong with any other
         weight is not None and bias is not None and x.is_cuda and x.dim() > 0 and x.dtype in TYPES and weight.dtype in TYPES
@@ -178,7 +180,7 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()
     if (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)
-            ) and torch.is_grad_enabled():
+            ) and torch.is_grad_enabled() or recorded():
         return _LayerNorm.apply(x, weight, bias, float(eps), keep)
     return _forward(x, weight, bias, float(eps), keep, False)[0]
 

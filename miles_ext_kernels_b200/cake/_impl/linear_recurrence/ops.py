@@ -16,12 +16,13 @@ from pathlib import Path
 from typing import Any
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.graph import increment_version
 
 from ..._runtime import loader, registry, workspace
 from ..gdn import native
 from ..gdn.native import pointer
-from ..rows import TYPES, check_device, on_device, once_differentiable
+from ..rows import TYPES, check_device, forward_mode, on_device, once_differentiable, recorded
 
 __all__ = ["check_supported", "gated_linear_recurrence", "gated_linear_recurrence_step", "prebuild", "release"]
 
@@ -121,8 +122,10 @@ def _gradients(ctx, dy, d_final):
 class _GatedLinearRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, g, h0, cu, want_final):
-        y, final, states = _forward(x, g, h0, cu, want_final, True)
-        ctx.save_for_backward(x, g, h0, cu, states)
+        train = any(ctx.needs_input_grad)
+        y, final, states = _forward(x, g, h0, cu, want_final, train)
+        if train:
+            ctx.save_for_backward(x, g, h0, cu, states)
         return y, final
 
     backward = staticmethod(once_differentiable(_gradients))
@@ -153,7 +156,7 @@ def gated_linear_recurrence(
     that ``cu_seqlens`` (``[N + 1]`` prefix sums of their lengths, on ``x``'s device, ``B = 1``) packs into the one row.
     A sequence may be empty: its state passes through.  Tokens behind the last sequence belong to none: their ``y`` and
     gradients are zero.  ``final_state``: FP32 ``[N, ...]`` when ``output_final_state``, else ``None``.  Not twice
-    differentiable."""
+    differentiable, and without a forward-mode derivative."""
     if x.dim() < 3:
         raise ValueError(f"linear_recurrence: x must be [B, T, ...channels]; got {tuple(x.shape)}")
     if g.shape != x.shape:
@@ -188,7 +191,8 @@ def gated_linear_recurrence(
     else:
         cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
         xv, gv = _rows(x), _rows(g)
-        if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or (h0 is not None and h0.requires_grad)):
+        if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or (h0 is not None and h0.requires_grad)
+                                        ) or recorded():
             y, final = _GatedLinearRecurrence.apply(xv, gv, h0, cu, bool(output_final_state))
         else:
             y, final, _ = _forward(xv, gv, h0, cu, output_final_state, False)
@@ -223,6 +227,11 @@ def _explain_step(x, g, state, state_indices):
     if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad or state.requires_grad):
         raise ValueError("linear_recurrence: the step updates its state in place and has no gradient; use "
                          "gated_linear_recurrence, or torch.no_grad()")
+    if forward_mode():
+        if any(unpack_dual(t).tangent is not None for t in (x, g, state)):
+            raise ValueError("linear_recurrence: the step updates its state in place and has no forward-mode derivative")
+    elif recorded():
+        raise ValueError("linear_recurrence: the step updates its state in place, which a trace would not hold")
     for name, t in (("g", g), ("state", state), ("state_indices", state_indices)):
         if t is not None and t.device != x.device:
             raise ValueError(f"linear_recurrence: {name} is on {t.device}, x on {x.device}")
@@ -248,6 +257,7 @@ def gated_linear_recurrence_step(x: torch.Tensor, g: torch.Tensor, state: torch.
         and state_indices.shape == shape[:1] and state_indices.device == device and 0 < shape[1] <= _MAX_CHANNELS
         and state.shape[0] > 0
         and not ((x.requires_grad or g.requires_grad or state.requires_grad) and torch.is_grad_enabled())
+        and not recorded()
     ):
         _explain_step(x, g, state, state_indices)
     rows, pool = shape[0], state.shape[0]

@@ -7,11 +7,13 @@ from contextlib import nullcontext
 from typing import Any
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable as _guarded
 
 from .._runtime import loader
 
-__all__ = ["CHECKPOINTS", "TYPES", "aligned", "check_device", "checkpoint_format", "on_device", "once_differentiable"]
+__all__ = ["CHECKPOINTS", "TYPES", "aligned", "check_device", "checkpoint_format", "forward_mode", "on_device",
+           "once_differentiable", "recorded"]
 
 # element types of the C ABI
 TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -19,6 +21,18 @@ TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 CHECKPOINTS = (None, "e4m3")
 
 _NOTHING = nullcontext()
+_tracing_state = torch._C._get_tracing_state
+
+
+def forward_mode() -> bool:
+    """Whether tensors may carry forward-mode tangents."""
+    return forward_ad._current_level >= 0
+
+
+def recorded() -> bool:
+    """Whether something besides the backward follows the call -- forward mode, a trace -- so that it has to go through its
+    autograd function even where nothing requires a gradient: the kernels work on addresses, which neither sees."""
+    return forward_ad._current_level >= 0 or _tracing_state() is not None
 
 
 def on_device(device: torch.device) -> Any:
