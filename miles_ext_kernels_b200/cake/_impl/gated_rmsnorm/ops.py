@@ -23,7 +23,7 @@ import torch
 from ..._runtime import config, loader, registry, workspace
 from ..gdn import native
 from ..gdn.native import pointer
-from ..rows import aligned, checkpoint_format, on_device, recorded
+from ..rows import aligned, checkpoint_format, on_device, once_differentiable, recorded
 
 __all__ = ["check_supported", "prebuild", "release", "rmsnorm_silu_gate"]
 
@@ -118,6 +118,7 @@ class _RmsnormSiluGate(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         *kept, weight = ctx.saved_tensors
         device = dy.device
@@ -154,7 +155,7 @@ def rmsnorm_silu_gate(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, ep
     place when its last stride is 1, its token and head strides are multiples of 8 elements and it is 16-byte aligned,
     else copied once (the same bits either way).  ``weight``: BF16 ``[128]``.  Returns BF16 ``y`` of ``x``'s shape;
     every gradient comes in BF16 and the weight gradient sums over the rows of this call only (reference:
-    ops.py:126-148).
+    ops.py:126-148).  Not twice differentiable.
 
     ``checkpoint`` (an extension of the reference's signature): ``None`` keeps ``x`` and ``z`` for the backward, ``"e4m3"``
     keeps ``x * rstd`` and ``z`` in 8 bits, each off by at most 2^-4 of its value (an ``x * rstd`` below 2^-6 by at

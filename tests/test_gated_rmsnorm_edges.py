@@ -120,3 +120,20 @@ def test_x_and_z_at_odd_addresses(checkpoint):
     one = torch.randn(2, 1159, device="cuda").bfloat16()[:1, 8:136]  # one row of a projection of odd width
     got = run(one, one, w, dy[:1, 0], checkpoint)
     assert all(torch.equal(a, b) for a, b in zip(got, run(one.clone(), one.clone(), w, dy[:1, 0], checkpoint)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_a_second_derivative_is_refused(checkpoint):
+    from miles_ext_kernels_b200.cake.gated_rmsnorm import rmsnorm_silu_gate
+
+    x, z, w, dy = make(6, 2, seed=3)
+    leaves = [t.requires_grad_() for t in (x, z, w)]
+    y = rmsnorm_silu_gate(*leaves, EPS, checkpoint=checkpoint)
+    grads = torch.autograd.grad(y, leaves, dy.requires_grad_(), create_graph=True)
+    first = [g.detach() for g in grads]
+    assert all(torch.equal(a, b) for a, b in zip(first, run(x, z, w, dy.detach(), checkpoint)[1:]))
+    # other paths of the sum have a second derivative; this one's must not be left out of it without a word
+    penalty = sum(g.float().square().sum() for g in grads) + x.float().pow(3).sum()
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        penalty.backward()
