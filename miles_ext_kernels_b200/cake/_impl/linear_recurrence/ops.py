@@ -6,8 +6,9 @@ Per channel, with ``a = exp(g)`` and the state of a sequence starting at ``h0`` 
     h[t] = a[t] h[t-1] + x[t],   y[t] = h[t]
     dh[t] = dy[t] + a[t+1] dh[t+1],   dx = dh,   dg[t] = dh[t] a[t] h[t-1],   dh0 = a[0] dh[0]
 
-States and sums in FP32, one rounding per output; a decay below e^-87.7, where FP32 ends, counts as zero.  The autograd node keeps ``x``, ``g`` and the FP32 state after every
-tile of 128 tokens; the backward recomputes the states inside a tile, so ``dg`` does not see a rounded ``y``.
+States and sums in FP32, one rounding per output; a decay below e^-86.98 = 1.67e-38, at FP32's end, counts as zero.  The
+autograd node keeps ``x``, ``g`` and the FP32 state after every tile of 128 tokens; the backward recomputes the states
+inside a tile, so ``dg`` does not see a rounded ``y``.
 """
 
 from __future__ import annotations

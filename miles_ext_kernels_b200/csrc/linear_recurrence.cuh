@@ -50,7 +50,7 @@ constexpr float kGlrReset = -1.0f;                   // A of a run that holds a 
 
 __device__ __forceinline__ float clamped(float g) {  // NaN stays
   float v;
-  asm("max.NaN.f32 %0, %1, 0fC2B00000;" : "=f"(v) : "f"(g));   // -88
+  asm("max.NaN.f32 %0, %1, 0fC2AE0000;" : "=f"(v) : "f"(g));   // -87
   asm("min.NaN.f32 %0, %1, 0f42B1999A;" : "=f"(v) : "f"(v));   // 88.8
   return v;
 }
@@ -60,8 +60,10 @@ __device__ __forceinline__ float clamped(float g) {  // NaN stays
 // 7e-6 with expf, 4e-7 with this.)  q of degree 4 is the minimax fit of (e^r - 1 - r) / r^2 over |r| <= log(2) / 2 in
 // the error of the whole, found by reweighted least squares: off by at most 5.3e-9, by 2e-10 for |r| < 0.05.  The
 // rounding of log 2 puts |n| 2e-9 into the relative error: at n = 1 the memory is a token long already.
-// n sits in the low bits of the shifted product, from where one multiply-add makes 2^n: for the clamped range between
-// n = -127, whose bits are zero (a gate at or below -88, minus infinity too, closes exactly), and n = 128, infinity.
+// n sits in the low bits of the shifted product, from where one multiply-add makes 2^(n - 1), for n from -126, whose bits are
+// zero (a gate at or below -87, minus infinity too, closes exactly), to 128; the factor is 2 (1 + p), the same rounding.
+// (With 2^n and 1 + p the last binade of FP32, gates from 88.38 to 88.72, would be infinite.  In its place the first one
+// goes: a decay below 2^-125.5 = e^-86.98 = 1.67e-38 is zero.)
 __device__ __forceinline__ Two decays(Two gates) {
   const float2 v = split(gates);
   const Two g = two(clamped(v.x), clamped(v.y)), shift = two(12582912.f);
@@ -71,10 +73,10 @@ __device__ __forceinline__ Two decays(Two gates) {
   q = fma2(q, r, two(0.0416662060f));
   q = fma2(q, r, two(0.166665182f));
   q = fma2(q, r, two(0.5f));
-  const Two e = add2(fma2(mul2(r, r), q, r), two(1.f));
+  const Two e = fma2(fma2(mul2(r, r), q, r), two(2.f), two(2.f));
   const float2 m = split(shifted);
-  return mul2(e, two(__int_as_float(__float_as_int(m.x) * (1 << 23) + 0x3f800000),
-                     __int_as_float(__float_as_int(m.y) * (1 << 23) + 0x3f800000)));
+  return mul2(e, two(__int_as_float(__float_as_int(m.x) * (1 << 23) + 0x3f000000),
+                     __int_as_float(__float_as_int(m.y) * (1 << 23) + 0x3f000000)));
 }
 
 __device__ __forceinline__ float fold(float A, float B, float h) { return A < 0.f ? B : fmaf(A, h, B); }

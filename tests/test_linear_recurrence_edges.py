@@ -36,3 +36,34 @@ def test_a_pool_that_a_graph_has_saved_and_that_is_then_stepped():
     with torch.inference_mode():
         pool = torch.zeros(4, 64, device="cuda")  # has no version
         assert torch.equal(step(x[:, 0], g[:, 0], pool), x[:, 0])
+
+
+def top_and_bottom():
+    """Gates whose decays reach both ends of FP32: up to the largest finite one, down past the smallest normal one."""
+    top = torch.linspace(88.0, 88.7228, 500)  # e^88.7228 = 3.4028e38
+    return torch.cat([top, -top, torch.linspace(-86.97, 88.0, 700), torch.tensor([-87.0, -200.0, -float("inf"), 89.0, 1e30])])
+
+
+@pytest.mark.gpu
+def test_decays_at_both_ends_of_fp32():
+    """One token from the state 1 (and, backwards, from the gradient 1): the decay itself.  It may be off by the rounding of
+    log 2, |n| 2e-9 for a gate of n log 2, and three half steps; below e^-86.98 it may be zero."""
+    from miles_ext_kernels_b200.cake.linear_recurrence import gated_linear_recurrence, gated_linear_recurrence_step as step
+
+    g = top_and_bottom().cuda()
+    want = g.double().exp()
+    h0, x = torch.ones(1, g.numel(), device="cuda"), torch.zeros(1, 1, g.numel(), device="cuda")
+    leaves = [t.requires_grad_() for t in (x, g[None, None].clone(), h0)]
+    y, _ = gated_linear_recurrence(*leaves)
+    _, dg, dh0 = torch.autograd.grad(y, leaves, torch.ones_like(y))
+    with torch.no_grad():
+        pool = torch.ones(1, g.numel(), device="cuda")
+        stepped = step(x[0], g[None], pool)
+    # (clamped, or the gate of minus infinity would make 0 * infinity of its bound, which is 0)
+    bound = want * (3 * 2.0**-24 + g.double().abs().clamp(max=200) / 0.693 * 2e-9) + torch.where(g < -86.98, 1.67e-38, 0.0).double()
+    for got in (y, dg, dh0, stepped, pool):
+        got = got.detach().flatten().double()
+        over = want > torch.finfo(FP32).max
+        assert torch.equal(got[over].isinf(), torch.ones_like(got[over]).bool()) and int(over.sum()) == 2
+        assert ((got - want).abs() <= bound)[~over].all()
+        assert (got[g <= -87.0] == 0).all()
