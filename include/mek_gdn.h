@@ -357,9 +357,11 @@ int mek_layer_norm_bwd(const void* dy, const void* x, int type, const uint8_t* c
  * More than mek_linear_recurrence_tile() tokens need states fp32 [2 batch tiles channels + 1], 16-byte aligned, with
  * tiles = ceil(tokens / tile): the state after every tile, which the backward reads; the backward needs scratch of the
  * same size.  Blocks of one launch wait for one another through them (in an order that cannot block, and for at most
- * a second: then the carried state is NaN), so no two calls that overlap may share them.  step: one token of every row on a pool of states fp32 [pool, channels] (state_row_stride elements
- * between them), updated in place: row r uses state slots[r] (int32, or int64 when slots_are_int64; NULL: r); a slot
- * outside [0, pool) leaves every state alone and gives zeros; rows that name one slot take their turns in row order.
+ * a second: then the carried state is NaN), so no two calls that overlap may share them.  A gate may be positive; a state
+ * that is not zero comes out infinite where a sequence grows by more than e^88 within 128 tokens.
+ * step: one token of every row on a pool of states fp32 [pool, channels] (state_row_stride elements between them), updated
+ * in place: row r uses state slots[r] (int32, or int64 when slots_are_int64; NULL: r); a slot outside [0, pool) leaves
+ * every state alone and gives zeros; rows that name one slot take their turns in row order.
  * No counterpart in the reference. */
 int mek_linear_recurrence_tile(void);
 int mek_linear_recurrence_fwd(const void* x, int x_type, const void* g, int g_type, void* y, int64_t batch,

@@ -152,12 +152,13 @@ def gated_linear_recurrence(
 
     ``x``: BF16, FP16 or FP32 ``[B, T, ...]``; every element of the trailing dimensions is a channel of its own.  ``g``:
     the log decay in nats, ``x``'s shape, in any of the three types (expand a gate that channels share; autograd sums
-    its gradient).  Both are read in place when the channels have unit stride, whatever the token and batch strides, else
-    copied once.  ``initial_state``: FP32 ``[N, ...]`` or ``None`` (zero); ``N`` is ``B``, or the number of sequences
-    that ``cu_seqlens`` (``[N + 1]`` prefix sums of their lengths, on ``x``'s device, ``B = 1``) packs into the one row.
-    A sequence may be empty: its state passes through.  Tokens behind the last sequence belong to none: their ``y`` and
-    gradients are zero.  ``final_state``: FP32 ``[N, ...]`` when ``output_final_state``, else ``None``.  Not twice
-    differentiable, and without a forward-mode derivative."""
+    its gradient).  A gate may be positive; a state that is not zero comes out infinite where a sequence grows by more
+    than e^88 within 128 tokens, FP32's range.  Both are read in place when the channels have unit stride, whatever the
+    token and batch strides, else copied once.  ``initial_state``: FP32 ``[N, ...]`` or ``None`` (zero); ``N`` is ``B``, or
+    the number of sequences that ``cu_seqlens`` (``[N + 1]`` prefix sums of their lengths, on ``x``'s device, ``B = 1``)
+    packs into the one row.  A sequence may be empty: its state passes through.  Tokens behind the last sequence belong to
+    none: their ``y`` and gradients are zero.  ``final_state``: FP32 ``[N, ...]`` when ``output_final_state``, else
+    ``None``.  Not twice differentiable, and without a forward-mode derivative."""
     if x.dim() < 3:
         raise ValueError(f"linear_recurrence: x must be [B, T, ...channels]; got {tuple(x.shape)}")
     if g.shape != x.shape:

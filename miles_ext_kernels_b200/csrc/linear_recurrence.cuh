@@ -79,11 +79,24 @@ __device__ __forceinline__ Two decays(Two gates) {
                      __int_as_float(__float_as_int(m.y) * (1 << 23) + 0x3f000000)));
 }
 
-__device__ __forceinline__ float fold(float A, float B, float h) { return A < 0.f ? B : fmaf(A, h, B); }
+// Gates may be positive, and a product of decays may then leave FP32's range where the states do not (kGrown): a state of
+// zero stays zero under any growth, and a run that holds a decay of zero is closed whatever grew before or after it.  (Growth
+// past the range from a state that is not zero is infinite.)  Folds wait for one another, so the two comparisons are only
+// made where an A is infinite, which a vote tells beforehand (in every fold: forward 231 -> 242 us, backward 416 -> 460).
+constexpr float kGlrInfinity = __builtin_huge_valf();
+template <bool kGrown>
+__device__ __forceinline__ float fold(float A, float B, float h) {
+  return A < 0.f ? B : fmaf(kGrown && A == kGlrInfinity && h == 0.f ? 0.f : A, h, B);
+}
+__device__ __forceinline__ float product(float A, float A2) {
+  const float p = A * A2;
+  return p != p && A == A && A2 == A2 ? 0.f : p;  // zero times infinity
+}
 // (A, B), then (A2, B2)
+template <bool kGrown>
 __device__ __forceinline__ void chain(float& A, float& B, float A2, float B2) {
-  B = fold(A2, B2, B);
-  A = A < 0.f || A2 < 0.f ? kGlrReset : A * A2;
+  B = fold<kGrown>(A2, B2, B);
+  A = A < 0.f || A2 < 0.f ? kGlrReset : kGrown ? product(A, A2) : A * A2;
 }
 
 // Where sequences lie: dense batches (cu = NULL: row b is sequence b, all T tokens) or one packed row.
@@ -145,7 +158,7 @@ struct GlrTensor {
   int64_t batch_stride, token_stride;
 };
 
-struct GlrShape {
+struct GlrShape {  // a __grid_constant__ of the kernels: the functions that are not inlined take its address, not a copy's
   Sequences seq;
   int batch, tokens, channels, tiles, channel_blocks;
   int window;        // words a warp looks back over at once; 0: one warp looks at the nearest four
@@ -173,6 +186,7 @@ struct GlrShared {
   int2 marks[kGlrWarps];                    // nearest word not set, nearest state, among the words a warp looked at
   GlrTileAt at, ahead;                      // the block's tile, and one to ask into L2 (tile < 0: none)
   int late;
+  int grown;                                // a warp's A is infinite or NaN
 };
 
 // The block's tile -- the next in order, or its own index where tiles do not wait for one another -- and the barriers.
@@ -189,7 +203,7 @@ __device__ __forceinline__ GlrTileAt take_tile(const GlrShape& s, GlrShared<kDir
       if (unsigned(index) >= gridDim.x) sh.at.tile = -1;
       sh.ahead = tile_at<kReverse>(s, min(index, int(gridDim.x) - 1 - s.ahead) + s.ahead);
       if (index >= int(gridDim.x) - s.ahead) sh.ahead.tile = -1;
-      sh.late = 0;
+      sh.late = sh.grown = 0;
     }
   }
   __syncthreads();
@@ -286,6 +300,11 @@ struct Words {  // of a lane's two channels
     return __float_as_uint(A0) != 0xffffffffu && __float_as_uint(A1) != 0xffffffffu;  // no operation makes this NaN
   }
   __device__ __forceinline__ bool state() const { return A0 < 0.f && A1 < 0.f; }
+  __device__ __forceinline__ bool finite() const { return A0 < kGlrInfinity && A1 < kGlrInfinity; }  // of A
+  template <bool kGrown>
+  __device__ __forceinline__ void onto(float (&h)[2]) const {
+    h[0] = fold<kGrown>(A0, B0, h[0]), h[1] = fold<kGrown>(A1, B1, h[1]);
+  }
 };
 __device__ __forceinline__ float* words_at(float* words, const GlrShape& s, const GlrTileAt& at, int tile) {
   return words + ((int64_t(at.b) * s.tiles + tile) * s.channels + at.c0 + 2 * (threadIdx.x & 31)) * 2;
@@ -342,9 +361,16 @@ __device__ __forceinline__ Two look_back(float* words, const GlrShape& s, const 
       ready = ready && __all_sync(0xffffffffu, v[k].set());
       if (!ready) break;
       if (__all_sync(0xffffffffu, v[k].state())) {
+        bool finite = true;
 #pragma unroll
-        for (int i = kGlrNear - 1; i >= 0; --i)
-          if (i <= k) h[0] = fold(v[i].A0, v[i].B0, h[0]), h[1] = fold(v[i].A1, v[i].B1, h[1]);
+        for (int i = 0; i < kGlrNear; ++i) finite = finite && (i > k || v[i].finite());
+        const bool grown = !__all_sync(0xffffffffu, finite);
+#pragma unroll
+        for (int i = kGlrNear - 1; i >= 0; --i) {
+          if (i > k) continue;
+          if (grown) v[i].template onto<true>(h);
+          else v[i].template onto<false>(h);
+        }
         return two(h[0], h[1]);
       }
     }
@@ -405,6 +431,11 @@ __device__ __forceinline__ void look_back_together(float* words, const GlrShape&
   }
   float h[2] = {0.f, 0.f};
   const int top = from / s.window;
+  bool finite = true;
+#pragma unroll
+  for (int k = 0; k < kGlrWindow; ++k)
+    if (k < s.window && warp * s.window + k <= from) finite = finite && v[k].finite();
+  const bool grown = !__all_sync(0xffffffffu, finite);
   for (int w = top; w >= 0; --w) {
     if (warp == w) {
       if (w < top) {
@@ -413,8 +444,10 @@ __device__ __forceinline__ void look_back_together(float* words, const GlrShape&
       }
 #pragma unroll
       for (int k = kGlrWindow - 1; k >= 0; --k)
-        if (k < s.window && w * s.window + k <= from)
-          h[0] = fold(v[k].A0, v[k].B0, h[0]), h[1] = fold(v[k].A1, v[k].B1, h[1]);
+        if (k < s.window && w * s.window + k <= from) {
+          if (grown) v[k].template onto<true>(h);
+          else v[k].template onto<false>(h);
+        }
       sh.carried[lane] = two(h[0], h[1]);
     }
     __syncthreads();
@@ -437,21 +470,51 @@ __device__ __forceinline__ Two carry_in(float* words, const GlrShape& s, const G
   }
   if (mine && !tile.state()) {  // else it was one already
     const float2 in = split(h);
-    publish<kPair>(words_at(words, s, at, at.tile), s, at,
-                   Words{kGlrReset, fold(tile.A0, tile.B0, in.x), kGlrReset, fold(tile.A1, tile.B1, in.y)});
+    float out[2] = {in.x, in.y};
+    tile.onto<true>(out);
+    publish<kPair>(words_at(words, s, at, at.tile), s, at, Words{kGlrReset, out[0], kGlrReset, out[1]});
   }
   if (before == 0 || s.window > 0) return h;
   if (mine) sh.carried[threadIdx.x & 31] = h;
   __syncthreads();
   return sh.carried[threadIdx.x & 31];
 }
+__device__ __forceinline__ Words words_of(const float4& v) { return {v.x, v.y, v.z, v.w}; }
+template <bool kGrown>
 __device__ __forceinline__ Two folded(const float4& v, Two h) {
   const float2 f = split(h);
-  return two(fold(v.x, v.y, f.x), fold(v.z, v.w, f.y));
+  return two(fold<kGrown>(v.x, v.y, f.x), fold<kGrown>(v.z, v.w, f.y));
 }
+template <bool kGrown>
 __device__ __forceinline__ void chain(Words& v, const float4& w) {
-  chain(v.A0, v.B0, w.x, w.y);
-  chain(v.A1, v.B1, w.z, w.w);
+  chain<kGrown>(v.A0, v.B0, w.x, w.y);
+  chain<kGrown>(v.A1, v.B1, w.z, w.w);
+}
+// A tile's pair, from its warps' in the order of time, and the state that enters warp `warp` when h enters the tile.
+template <bool kReverse, bool kGrown>
+__device__ __forceinline__ Words chained(const float4 (*pair)[32]) {
+  const int lane = threadIdx.x & 31;
+  Words tile = words_of(pair[kReverse ? kGlrWarps - 1 : 0][lane]);
+#pragma unroll
+  for (int i = 1; i < kGlrWarps; ++i) chain<kGrown>(tile, pair[kReverse ? kGlrWarps - 1 - i : i][lane]);
+  return tile;
+}
+template <bool kReverse, bool kGrown>
+__device__ __forceinline__ Two entering(const float4 (*pair)[32], int warp, Two h) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kGlrWarps - 1; ++i) {
+    const int w = kReverse ? kGlrWarps - 1 - i : i;
+    if (kReverse ? w > warp : w < warp) h = folded<kGrown>(pair[w][lane], h);
+  }
+  return h;
+}
+// The same where an A is infinite or NaN.
+template <bool kReverse>
+static __device__ __noinline__ Words chained_grown(const float4 (*pair)[32]) { return chained<kReverse, true>(pair); }
+template <bool kReverse>
+static __device__ __noinline__ Two entering_grown(const float4 (*pair)[32], int warp, Two h) {
+  return entering<kReverse, true>(pair, warp, h);
 }
 
 // A warp's gates and, once they are exponentiated, its decays [16][64] in FP32, in one place.  16-bit gates arrive in the
@@ -548,12 +611,25 @@ __device__ __noinline__ Two fold_from_ends(const float* decay, X* ds, uint32_t e
   }
   return D;
 }
+// Whether a lane's product of decays left FP32's range or met a NaN; the same for the whole warp.  The walk's A, and its D,
+// which takes such products times gradients of zero, are then folded once more.
+__device__ __forceinline__ bool overflowed(Two A) {
+  const float2 a = split(A);
+  return __any_sync(0xffffffffu, !(a.x < kGlrInfinity && a.y < kGlrInfinity));
+}
+static __device__ __noinline__ Two product_of(const float* decay) {
+  float2 A = make_float2(1.f, 1.f);
+#pragma unroll 1
+  for (int j = 0; j < kGlrTokens; ++j) {
+    const float2 a = split(decay_at(decay, j));
+    A = make_float2(product(A.x, a.x), product(A.y, a.y));
+  }
+  return two(A.x, A.y);
+}
 __device__ __forceinline__ float4 packed(Two A, Two B) {
   const float2 a = split(A), b = split(B);
   return make_float4(a.x, b.x, a.y, b.y);
 }
-__device__ __forceinline__ Words words_of(const float4& v) { return {v.x, v.y, v.z, v.w}; }
-
 // ---- host ------------------------------------------------------------------------------------------------------------
 inline int check_glr(const char* what, int x_type, int g_type, int64_t batch, int64_t tokens, int64_t channels, int64_t seqs,
               const void* cu) {

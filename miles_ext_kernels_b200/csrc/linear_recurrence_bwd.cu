@@ -17,7 +17,7 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
                                                                     const __grid_constant__ CUtensorMap g_map,
                                                                     const __grid_constant__ CUtensorMap dx_map,
                                                                     const __grid_constant__ CUtensorMap dg_map,
-                                                                    const GlrBwdArgs p, const GlrShape s) {
+                                                                    const GlrBwdArgs p, const __grid_constant__ GlrShape s) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ GlrShared<2> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -66,11 +66,13 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
       if (edges.kind == kInside) walk_tokens<X, G, true, false>(decay, xs, ds, edges, s0, d1, A, B, D);
       else walk_tokens<X, G, true, true>(decay, xs, ds, edges, s0, d1, A, B, D);
     }
-    Two R = A;
-    if (edges.kind == kManyEdges) {
-      if (edges.starts) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
-      if (edges.ends) D = fold_from_ends<X, kTma>(decay, ds, edges.ends, p.d_final, s, at, t0);
+    const bool grown = overflowed(A);
+    if (edges.kind == kManyEdges || grown) {
+      if (grown) A = product_of(decay), sh.grown = 1;
+      if (edges.kind == kManyEdges && edges.starts) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
+      if (edges.ends || grown) D = fold_from_ends<X, kTma>(decay, ds, edges.ends, p.d_final, s, at, t0);
     }
+    Two R = A;
     if (edges.starts) A = two(kGlrReset);
     if (edges.ends) R = two(kGlrReset);
     if (!arrived) A = R = two(kGlrReset), B = D = lost();
@@ -79,20 +81,21 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 3) glr_bwd_kernel(const __grid
   }
   __syncthreads();
   if (s.tiles > 1) {
-    Words tile = words_of(sh.pair[1][kGlrWarps - 1][lane]);
+    Words tile;
     if (warp == kGlrWarps - 1) {
-#pragma unroll
-      for (int w = kGlrWarps - 2; w >= 0; --w) chain(tile, sh.pair[1][w][lane]);
+      tile = chained<true, false>(sh.pair[1]);
+      if (!__all_sync(0xffffffffu, tile.finite() && sh.grown == 0)) tile = chained_grown<true>(sh.pair[1]);
       publish<kTma>(words_at(p.words, s, at, at.tile), s, at, tile);
     }
     c = carry_in<kTma, true>(p.words, s, at, sh, kGlrWarps - 1, tile);
   }
-#pragma unroll
-  for (int w = 0; w < kGlrWarps - 1; ++w)
-    if (w < warp) h = folded(sh.pair[0][w][lane], h);
-#pragma unroll
-  for (int w = kGlrWarps - 1; w > 0; --w)
-    if (w > warp) c = folded(sh.pair[1][w][lane], c);
+  if (sh.grown == 0) {
+    h = entering<false, false>(sh.pair[0], warp, h);
+    c = entering<true, false>(sh.pair[1], warp, c);
+  } else {
+    h = entering_grown<false>(sh.pair[0], warp, h);
+    c = entering_grown<true>(sh.pair[1], warp, c);
+  }
   if (!arrived) h = c = lost();
   if (!any) return;
   // forward once more for the state before every token, then back with the adjoint; dx takes dy's place, dg the gates'

@@ -13,7 +13,7 @@ template <typename X, typename G, bool kTma>
 __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid_constant__ CUtensorMap x_map,
                                                                     const __grid_constant__ CUtensorMap g_map,
                                                                     const __grid_constant__ CUtensorMap y_map,
-                                                                    const GlrFwdArgs p, const GlrShape s) {
+                                                                    const GlrFwdArgs p, const __grid_constant__ GlrShape s) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ GlrShared<1> sh;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -50,24 +50,26 @@ __global__ void __launch_bounds__(kGlrWarps * 32, 4) glr_fwd_kernel(const __grid
     if (edges.kind == kInside) walk_tokens<X, G, false, false>(decay, xs, xs, edges, none, none, A, B, no_adjoint);
     else walk_tokens<X, G, false, true>(decay, xs, xs, edges, s0, none, A, B, no_adjoint);
   }
-  if (edges.kind == kManyEdges) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
+  const bool grown = overflowed(A);
+  if (edges.kind == kManyEdges || grown) {
+    if (grown) A = product_of(decay), sh.grown = 1;
+    if (edges.kind == kManyEdges) B = fold_from_starts<X, kTma>(decay, xs, edges.starts, p.h0, s, at, t0);
+  }
   if (edges.starts) A = two(kGlrReset);
   if (!arrived) A = two(kGlrReset), B = lost();
   sh.pair[0][warp][lane] = packed(A, B);
   __syncthreads();
   Two h = two(0.f);
   if (s.tiles > 1) {
-    Words tile = words_of(sh.pair[0][0][lane]);
+    Words tile;
     if (warp == 0) {
-#pragma unroll
-      for (int w = 1; w < kGlrWarps; ++w) chain(tile, sh.pair[0][w][lane]);
+      tile = chained<false, false>(sh.pair[0]);
+      if (!__all_sync(0xffffffffu, tile.finite() && sh.grown == 0)) tile = chained_grown<false>(sh.pair[0]);
       publish<kTma>(words_at(p.words, s, at, at.tile), s, at, tile);
     }
     h = carry_in<kTma, false>(p.words, s, at, sh, 0, tile);
   }
-#pragma unroll
-  for (int w = 0; w < kGlrWarps - 1; ++w)
-    if (w < warp) h = folded(sh.pair[0][w][lane], h);
+  h = sh.grown == 0 ? entering<false, false>(sh.pair[0], warp, h) : entering_grown<false>(sh.pair[0], warp, h);
   if (!arrived) h = lost();
   if (!any) return;
   if (edges.kind == kInside) {

@@ -73,7 +73,8 @@ def linear_recurrence(x, g, lengths, h0=None, dy=None, d_final=None):
     token in 64 bits.  The slack follows the sizes: with m the sum of magnitudes that the state could have (no
     cancellation), a step adds at most 6 half steps of FP32 to what it carries over -- a decay within 3 half steps of
     exp(g), its product and the fold's -- and 2 to the new state.  A decay below 2^-125.5 counts as zero, which takes
-    away less than 2^-125.5 = 1.663e-38 of what the step carries over (2^-126 = 1.1755e-38, times 2^0.5)."""
+    away less than 2^-125.5 = 1.663e-38 of what the step carries over (2^-126 = 1.1755e-38, times 2^0.5), and no
+    more than the decay itself."""
     total, channels = x.shape
     x, a = x.double(), g.double().exp()
     n = len(lengths)
@@ -88,7 +89,7 @@ def linear_recurrence(x, g, lengths, h0=None, dy=None, d_final=None):
         h, m, e = h0[i], h0[i].abs(), torch.zeros_like(h0[i])
         for t in range(start, start + length):
             before[t], before_slack[t] = h, e
-            e = a[t] * (e + 6 * U32 * m) + 1.67e-38 * m
+            e = a[t] * (e + 6 * U32 * m) + a[t].clamp(max=1.67e-38) * m
             h, m = a[t] * h + x[t], a[t] * m + x[t].abs()
             e = e + 2 * U32 * m
             y[t], dy_slack[t] = h, e
@@ -108,7 +109,7 @@ def linear_recurrence(x, g, lengths, h0=None, dy=None, d_final=None):
             e = e + 2 * U32 * m
             dx[t], dx_slack[t] = dh, e
             c = a[t] * dh
-            e, m = a[t] * (e + 6 * U32 * m) + 1.67e-38 * m, a[t] * m
+            e, m = a[t] * (e + 6 * U32 * m) + a[t].clamp(max=1.67e-38) * m, a[t] * m
             dg[t] = c * before[t]
             dg_slack[t] = e * before[t].abs() + c.abs() * before_slack[t] + e * before_slack[t] + 4 * U32 * dg[t].abs()
         dh0[i], dh0_slack[i] = c, e

@@ -67,3 +67,48 @@ def test_decays_at_both_ends_of_fp32():
         assert torch.equal(got[over].isinf(), torch.ones_like(got[over]).bool()) and int(over.sum()) == 2
         assert ((got - want).abs() <= bound)[~over].all()
         assert (got[g <= -87.0] == 0).all()
+
+
+def growth(kind, tokens, channels):
+    """Gates that grow past FP32's range inside a tile, and where there is something to grow."""
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.zeros(1, tokens, channels, device="cuda")
+    dy = torch.zeros(1, tokens, channels, device="cuda")
+    g = torch.full((1, tokens, channels), 8.0 if kind == "in a warp" else 1.0, device="cuda")
+    randn = lambda n: torch.randn(n, channels, device="cuda", generator=gen)  # noqa: E731
+    if kind == "closed after it":  # what grew is gone behind a gate of minus infinity
+        g[:, 150] = -float("inf")
+        g[:, 151:] = -0.1
+        x[:, 150:], dy[:, 170:] = randn(tokens - 150), randn(tokens - 170)
+    elif kind == "closed before it":
+        g[:, :40] = -0.1
+        g[:, 40] = -float("inf")
+        x[:, :20], dy[:, :30] = randn(20), randn(30)
+        g[:, 41:] = 2.0
+    else:
+        reach = 8 if kind == "in a warp" else 60
+        x[:, -reach:], dy[:, :reach] = randn(reach), randn(reach)
+    return x, g, dy
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("channels", [64, 33, 640, 12800])
+@pytest.mark.parametrize("kind", ["in a tile", "in a warp", "closed after it", "closed before it"])
+def test_growth_of_nothing_is_nothing(kind, channels):
+    from miles_ext_kernels_b200.cake.linear_recurrence import gated_linear_recurrence
+    from oracle import rows_oracle as R
+
+    tokens = 900
+    x, g, dy = growth(kind, tokens, channels)
+    leaves = [t.clone().requires_grad_() for t in (x, g)]
+    y, final = gated_linear_recurrence(*leaves, output_final_state=True)
+    dl = torch.zeros_like(final)
+    if kind == "closed after it":
+        dl.normal_()
+    dx, dg = torch.autograd.grad((y, final), leaves, (dy, dl))
+    some = slice(0, 70)  # the channels are alike
+    want = R.linear_recurrence(x[0, :, some], g[0, :, some], [tokens], None, dy[0, :, some], dl[:, some])
+    for name, got in (("y", y[0]), ("final", final), ("dx", dx[0]), ("dg", dg[0])):
+        got = got.detach()
+        assert torch.isfinite(got).all(), name
+        assert R.misses(got[:, some], *want[name]) == 0, name
