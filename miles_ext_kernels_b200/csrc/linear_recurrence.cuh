@@ -130,8 +130,6 @@ __device__ __forceinline__ int sequence_of(const Sequences& s, int b, int t) {
 struct Span {
   uint32_t bounds;
   int lo, hi;
-  __device__ __forceinline__ bool starts(int j) const { return (bounds >> j) & 1; }
-  __device__ __forceinline__ bool ends(int j) const { return (bounds >> (j + 1)) & 1; }
 };
 __device__ __forceinline__ Span span_of(const Sequences& s, int t0) {
   Span span{0u, 0, s.tokens};
