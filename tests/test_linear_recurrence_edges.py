@@ -112,3 +112,63 @@ def test_growth_of_nothing_is_nothing(kind, channels):
         got = got.detach()
         assert torch.isfinite(got).all(), name
         assert R.misses(got[:, some], *want[name]) == 0, name
+
+
+PACKED = [
+    ([1], 0), ([0, 5], 0), ([1] * 70, 0), ([3] * 200, 5), ([0, 0, 3, 0, 0, 130, 0, 1, 16, 0], 0), ([16, 16, 32, 64], 7),
+    ([300, 2, 255], 40), ([0] * 45 + [20] + [0] * 45, 0), ([7, 0, 5, 1, 2, 0, 0, 1, 200, 9, 300, 1, 1], 130), ([513], 600),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,tail", PACKED)
+@pytest.mark.parametrize("channels,dtype,gdtype", [(128, BF16, FP32), (128, BF16, BF16), (72, torch.float16, torch.float16),
+                                                   (64, FP32, BF16), (64, FP32, FP32)])
+def test_packed_sequences_that_come_by_boxes(lengths, tail, channels, dtype, gdtype):
+    """Channels that TMA can address: several boundaries in a warp, empty sequences, tokens behind the last one, and gates
+    of 16 bits, whose gradients take the place of decays."""
+    import test_linear_recurrence as base
+
+    total = sum(lengths) + tail
+    x, g, h0, dy, dl = base.make(1, total, channels, dtype, gdtype, len(lengths), seed=21)
+    if tail:
+        x[:, total - tail :], dy[:, total - tail :] = float("nan"), float("inf")
+    cu = torch.tensor([0] + lengths, device="cuda").cumsum(0).int()
+    base.check(base.run(x, g, h0, dy, dl, cu), x, g, h0, dy, dl, lengths, str(lengths)[:40], tail)
+    base.check(base.run(x, g, None, dy, None, cu, final=False), x, g, None, dy, None, lengths, "no states", tail)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gdtype", [FP32, BF16])
+@pytest.mark.parametrize("kind", ["mixed", "open"])
+@pytest.mark.parametrize("chains", [1, 16, 20, 30, 50, 100, 400])
+def test_every_depth_of_the_look_back(chains, kind, gdtype):
+    """How far a block looks back follows from the number of chains (channel blocks x batch rows): 48 tiles, 5 x 8, ... 8, four by
+    one warp.  With open gates a state carried wrongly would show; a chain has the bits that it has alone."""
+    import test_linear_recurrence as base
+
+    tokens, batch = 128 * 14 + 37, 2 if chains % 20 == 0 else 1
+    channels = 64 * chains // batch
+    x, g, h0, dy, dl = base.make(batch, tokens, channels, BF16, gdtype, batch, kind, seed=22)
+    got = base.run(x, g, h0, dy, dl)
+    for row, block in {(0, 0), (batch - 1, channels // 64 - 1)}:
+        some, one = slice(64 * block, 64 * block + 64), slice(row, row + 1)
+        part = [t[one][..., some].contiguous() for t in (x, g, h0, dy, dl)]
+        mine = {n: t[one][..., some].contiguous() for n, t in got.items()}
+        base.check(mine, *part, [tokens], f"{chains} chains")
+        alone = base.run(*part)
+        assert all(torch.equal(mine[n], alone[n]) for n in alone)
+
+
+@pytest.mark.gpu
+def test_a_gradient_at_an_odd_address():
+    import test_linear_recurrence as base
+
+    x, g, h0, dy, dl = base.make(2, 200, 64, BF16, BF16, 2, seed=23)
+    want = base.run(x, g, h0, dy, dl)
+    for offset in (1, 4):
+        flat = torch.empty(dy.numel() + offset, device="cuda", dtype=BF16)
+        states = torch.empty(dl.numel() + 1, device="cuda")
+        moved, moved_states = flat[offset:].view(dy.shape).copy_(dy), states[1:].view(dl.shape).copy_(dl)
+        got = base.run(x, g, h0, moved, moved_states)
+        assert moved.is_contiguous() and all(torch.equal(got[n], want[n]) for n in want)
