@@ -307,7 +307,7 @@ int mek_gated_rmsnorm_bwd_kept(const void* dy, const uint8_t* n_codes, const uin
 /* ------------------------------------------------------------------------------------------------------------------
  * Packed causal depthwise conv1d (kernel size 4) + SiLU, the short convolution in front of the GDN / KDA op:
  *     pre[t, c] = sum_{k<4} w[c, k] x[t - 3 + k, c] (inside t's document),   y = bf16(pre sigmoid(pre))
- * x, y, dy, dx bf16 [tokens, channels] dense (channels a multiple of 8); weight [channels, 4] fp32, or bf16 when
+ * x, y, dy, dx bf16 [tokens, channels] dense, 16-byte aligned (channels a multiple of 8); weight [channels, 4] fp32, or bf16 when
  * weight_is_bf16; reach uint8 [tokens] from mek_conv1d_reach (cu_seqlens int32 [num_docs + 1] on the device).
  * Backward: SiLU' at the BF16-rounded preactivation, or at the unrounded one with FP64 weight-gradient sums when
  * fp32_policy; dw in the weight's dtype (or NULL with dw_partial NULL); dw_partial holds

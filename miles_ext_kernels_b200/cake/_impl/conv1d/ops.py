@@ -16,6 +16,7 @@ import torch
 
 from ..._runtime import config, loader, registry, workspace
 from ..gdn import native
+from ..rows import aligned
 
 __all__ = ["causal_conv1d", "causal_conv1d_kcp", "causal_conv1d_kcp_multi", "check_supported", "prebuild", "release"]
 
@@ -126,7 +127,7 @@ class _CausalConv1d(torch.autograd.Function):
         xs, weights, kept = saved[:n], saved[n : 2 * n], list(saved[2 * n :])
         reaches = [kept.pop(0) if have else None for have in ctx.have_reach]
         device = xs[0].device
-        dys = [torch.zeros_like(x) if dy is None else dy.reshape(x.shape).to(torch.bfloat16).contiguous()
+        dys = [torch.zeros_like(x) if dy is None else aligned(dy.reshape(x.shape).to(torch.bfloat16))
                for x, dy in zip(xs, dys)]
         reachable = KERNEL_SIZE - 1
         widths = [x.shape[1] for x in xs]
@@ -177,7 +178,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, cu_seqlens: torch.Tenso
                   silu_grad_preactivation: str | None = None) -> torch.Tensor:
     """Autograd-enabled ``silu(causal depthwise conv1d)`` of the packed documents of ``x``.
 
-    ``x``: BF16 ``[1, S, C]`` or ``[S, C]`` (copied once when not contiguous); ``weight``: FP32 or BF16 ``[C, 4]``;
+    ``x``: BF16 ``[1, S, C]`` or ``[S, C]`` (copied once when not contiguous or not 16-byte aligned); ``weight``: FP32 or BF16 ``[C, 4]``;
     ``cu_seqlens``: ``[num_docs + 1]`` prefix sums of the document lengths on ``x``'s device (``None``: one
     document, built on the device).  ``silu_grad_preactivation`` (``bf16`` / ``fp32``) defaults to the configured
     policy, read now.  Returns BF16 ``y`` of ``x``'s shape; the weight gradient comes in ``weight``'s dtype
@@ -190,7 +191,7 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, cu_seqlens: torch.Tenso
     _checked(x, weight)
     config.variant(OP)
     policy = _policy(silu_grad_preactivation)
-    x = x.contiguous()
+    x = aligned(x)
     tokens = x.shape[-2]
     if cu_seqlens is None:
         cu_seqlens = torch.arange(2, dtype=torch.int32, device=x.device).mul_(tokens)  # no host copy, no sync
@@ -271,7 +272,7 @@ def causal_conv1d_kcp_multi(xs, weights, kcp_context: Any, *, recompute_handle: 
     policy = _policy(None)
     tokens = int(kcp_context.num_tokens)
     shapes = [x.shape for x in xs]
-    xs = [x.contiguous().view(-1, x.shape[-1]) for x in xs]
+    xs = [aligned(x).view(-1, x.shape[-1]) for x in xs]
     if any(x.shape[0] != tokens for x in xs):
         raise ValueError(f"causal_conv1d_kcp: the context holds {tokens} tokens on this rank, the tensors "
                          f"{[x.shape[0] for x in xs]}")

@@ -19,6 +19,7 @@ from typing import Any
 import torch
 
 from ..._runtime import config, loader, registry
+from ..rows import aligned
 from . import meta as meta_module
 from . import native, stages
 from . import tape as tape_module
@@ -174,24 +175,24 @@ def _no_tokens(q, k, v, g, beta, initial_state, output_final_state, cu_seqlens):
 # autograd
 # --------------------------------------------------------------------------------------------------------------------
 def _packed(x: torch.Tensor) -> torch.Tensor:
-    """``[B, T, heads, ...]`` -> contiguous ``[B * T, heads, ...]`` (a view when x is contiguous)."""
-    return x.contiguous().view(x.shape[0] * x.shape[1], *x.shape[2:])
+    """``[B, T, heads, ...]`` -> contiguous ``[B * T, heads, ...]`` (a view when x is contiguous and 16-byte aligned)."""
+    return aligned(x).view(x.shape[0] * x.shape[1], *x.shape[2:])
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``[B, T, heads, 128]`` -> ``[B * T, heads, 128]`` without a copy when x is dense or a column slice of a wider
     packed row (heads contiguous inside a token, tokens a fixed stride apart, 16-byte aligned): the kernels take the
-    token stride.  Anything else is made contiguous first."""
+    token stride.  Anything else is copied first."""
     B, T = x.shape[0], x.shape[1]
     if x.is_contiguous():
-        return x.view(B * T, *x.shape[2:])
+        return _packed(x)
     pitch = x.stride(1)
     sliced = (
         x.stride(3) == 1 and x.stride(2) == HEAD_DIM and pitch >= x.shape[2] * HEAD_DIM and pitch % 8 == 0
         and (B == 1 or x.stride(0) == T * pitch) and x.data_ptr() % 16 == 0
     )
     if not sliced:
-        return x.contiguous().view(B * T, *x.shape[2:])
+        return _packed(x)
     return x.as_strided((B * T, x.shape[2], HEAD_DIM), (pitch, HEAD_DIM, 1))
 
 
@@ -226,7 +227,7 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
             if qp.stride(0) != kp.stride(0):  # the kernels take one token stride for q and k
                 qp, kp = qp.contiguous(), kp.contiguous()
             ctx.packed_grads = _tile_one_row(qp, kp, vp)
-            h0 = None if initial_state is None else initial_state.detach().float().contiguous()
+            h0 = None if initial_state is None else aligned(initial_state.detach().float())
             want_final = bool(output_final_state)
             ctx.scan_segments = _scan_segments()
             # under context parallelism the exchange supplies the state at this rank's start and takes the one at
@@ -255,7 +256,7 @@ class ChunkGatedDeltaRuleFunction(torch.autograd.Function):
             if do is None:
                 do = torch.zeros(v_shape, dtype=torch.bfloat16, device=device)
             dop = _packed(do if do.dtype == torch.bfloat16 else do.bfloat16())
-            dhtp = None if dht is None else dht.float().contiguous()
+            dhtp = None if dht is None else aligned(dht.float())
             want_dh0 = ctx.has_initial_state
             dq, dk, dv, dg, dbeta, dh0 = stages.backward(tape, meta, ctx.scale, dop, dhtp, kept["h0"], want_dh0,
                                                                scan_segments=ctx.scan_segments, exchange=ctx.exchange,

@@ -39,6 +39,7 @@ import torch
 from ..._runtime import config
 from ..gdn import tape as tape_module
 from ..gdn.kcp import KcpContext
+from ..rows import aligned
 from . import ops
 
 __all__ = [
@@ -168,7 +169,7 @@ def _context(ctx: Any) -> KcpContext:
 
 
 def _shard(q, k, v, g, beta, ctx: KcpContext):
-    q3, k3, v3, g3 = (ops._packed3(t, n).contiguous() for t, n in ((q, "q"), (k, "k"), (v, "v"), (g, "g")))
+    q3, k3, v3, g3 = (aligned(ops._packed3(t, n)) for t, n in ((q, "q"), (k, "k"), (v, "v"), (g, "g")))
     beta3 = ops._packed_beta(beta)
     g3 = g3 if g3.dtype == torch.float32 else g3.float()
     ops._check(q3, k3, v3, g3, beta3, ctx.cu_seqlens)
@@ -272,7 +273,7 @@ class _ChunkKdaKcp(torch.autograd.Function):
     def backward(fn, do):
         shape, g_shape, beta_shape = fn.shapes
         scale, l2norm, options = fn.call
-        do3 = ops._packed3(do, "dout").contiguous().to(torch.bfloat16)
+        do3 = aligned(ops._packed3(do, "dout").to(torch.bfloat16))
         saved, kept = tape_module.restore(fn)
         if isinstance(saved, _LightTape):  # replay this rank's kernels from the states the forward received
             _, saved = _forward_local(saved.q, saved.k, kept["v"], saved.g, kept["beta32"], fn.kcp, scale, l2norm,
@@ -328,9 +329,9 @@ def chunk_kda_bwd_kcp(q, k, v, g, beta, ctx, dout, *, saved=None, scale=None, us
         _, saved = chunk_kda_fwd_kcp(q, k, v, g, beta, ctx, scale=scale, use_gate_in_kernel=use_gate_in_kernel,
                                      A_log=A_log, dt_bias=dt_bias, lower_bound=lower_bound,
                                      use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel, **options)
-    v3 = ops._packed3(v, "v").contiguous()
+    v3 = aligned(ops._packed3(v, "v"))
     beta32 = ops._packed_beta(beta).float().contiguous()
-    do3 = ops._packed3(dout, "dout").contiguous().to(torch.bfloat16)
+    do3 = aligned(ops._packed3(dout, "dout").to(torch.bfloat16))
     with torch.no_grad():
         dq, dk, dv, dg, dbeta = _backward_kcp(saved, v3, beta32, do3, ctx, chosen.exchange)
     grads = [dq.view(q.shape), dk.view(q.shape), dv.view(v.shape), dbeta.view(beta.shape).to(beta_dtype),

@@ -26,6 +26,7 @@ from ..gdn import meta as meta_module
 from ..gdn import native, scan
 from ..gdn import tape as tape_module
 from ..gdn.stages import check_status, dims_of
+from ..rows import aligned
 
 OP = "kda"
 HEAD_DIM = 128
@@ -267,7 +268,7 @@ class _ChunkKda(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, cu_seqlens, scale, use_qk_l2norm, cu_seqlens_cpu=None):
         shape = q.shape
-        q3, k3, v3, g3 = (_packed3(t, n).contiguous() for t, n in ((q, "q"), (k, "k"), (v, "v"), (g, "g")))
+        q3, k3, v3, g3 = (aligned(_packed3(t, n)) for t, n in ((q, "q"), (k, "k"), (v, "v"), (g, "g")))
         beta3 = _packed_beta(beta)
         g3 = g3 if g3.dtype == F32 else g3.float()
         _check(q3, k3, v3, g3, beta3, cu_seqlens)
@@ -283,7 +284,7 @@ class _ChunkKda(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         shape, g_shape, beta_shape = ctx.shapes
-        do3 = _packed3(do, "dout").contiguous()
+        do3 = aligned(_packed3(do, "dout"))
         if do3.dtype != BF16:
             do3 = do3.to(BF16)
         saved, kept = tape_module.restore(ctx)
@@ -323,7 +324,7 @@ def chunk_kda_fwd(q, k, v, g, beta, cu_seqlens, *, scale=None, save_for_backward
     v, beta = seam(v, beta)
     with torch.no_grad():
         gate = _gate(g, use_gate_in_kernel, A_log, dt_bias, lower_bound)
-        q3, k3, v3, g3 = (_packed3(t, n).contiguous() for t, n in ((q, "q"), (k, "k"), (v, "v"), (gate, "g")))
+        q3, k3, v3, g3 = (aligned(_packed3(t, n)) for t, n in ((q, "q"), (k, "k"), (v, "v"), (gate, "g")))
         beta3 = _packed_beta(beta)
         _check(q3, k3, v3, g3, beta3, cu_seqlens)
         with torch.cuda.device(q.device):
@@ -344,9 +345,9 @@ def chunk_kda_bwd(q, k, v, g, beta, cu_seqlens, dout, *, saved=None, scale=None,
         _, saved = chunk_kda_fwd(q, k, v, g, beta, cu_seqlens, scale=scale, use_gate_in_kernel=use_gate_in_kernel,
                                  A_log=A_log, dt_bias=dt_bias, lower_bound=lower_bound,
                                  use_qk_l2norm_in_kernel=use_qk_l2norm_in_kernel)
-    v3 = _packed3(v, "v").contiguous()
+    v3 = aligned(_packed3(v, "v"))
     beta3 = _packed_beta(beta)
-    do3 = _packed3(dout, "dout").contiguous().to(BF16)
+    do3 = aligned(_packed3(dout, "dout").to(BF16))
     with torch.no_grad(), torch.cuda.device(v.device):
         dq, dk, dv, dg, dbeta, _ = _backward(saved, v3, beta3.float().contiguous(), do3)
     grads = [dq.view(q.shape), dk.view(q.shape), dv.view(v.shape), dbeta.view(beta.shape).to(beta_dtype),

@@ -12,6 +12,7 @@
 // document; dw[c, k] = sum_t dpre[t] x[t - 3 + k].  The weight gradient is summed in a fixed order: per run in
 // registers (FP32; under the fp32 policy FP32 over four tokens, then FP64), then over the runs in FP64 by a second launch.  The number of runs is
 // a function of the token count alone: identical inputs give identical bits.
+#include <initializer_list>
 #include <type_traits>
 
 #include "common.cuh"
@@ -379,11 +380,13 @@ ConvPlan conv_plan(int tokens) {
   return {(tokens + run_len - 1) / run_len, run_len};
 }
 
-int check_conv(const char* what, int tokens, int channels, int num_docs) {
+int check_conv(const char* what, int tokens, int channels, int num_docs, std::initializer_list<const void*> rows) {
   using namespace mek;
   if (tokens <= 0 || num_docs <= 0) return fail(MEK_ERR_INVALID, "%s: no tokens or no documents", what);
   if (channels <= 0 || channels % 8 != 0)
     return fail(MEK_ERR_INVALID, "%s: the channel count must be a positive multiple of 8, got %d", what, channels);
+  for (const void* p : rows)  // read and written as words
+    if (reinterpret_cast<uintptr_t>(p) % 16 != 0) return fail(MEK_ERR_INVALID, "%s: rows must be 16-byte aligned", what);
   return MEK_OK;
 }
 
@@ -406,7 +409,7 @@ int mek_conv1d_fwd(const void* x, const void* x_prev, const void* weight, int we
                    void* y, int tokens, int channels, void* stream) {
   using namespace mek;
   if (!x || !weight || !reach || !y) return fail(MEK_ERR_INVALID, "conv1d_fwd: a null pointer");
-  if (int rc = check_conv("conv1d_fwd", tokens, channels, 1)) return rc;
+  if (int rc = check_conv("conv1d_fwd", tokens, channels, 1, {x, x_prev, y})) return rc;
   const ConvPlan plan = conv_plan(tokens);
   constexpr int kFwdCh = 4;  // channels per thread
   const dim3 grid(plan.runs, (channels + 256 * kFwdCh - 1) / (256 * kFwdCh));
@@ -431,7 +434,7 @@ int mek_conv1d_bwd(const void* x, const void* x_prev, const void* x_next, const 
     return fail(MEK_ERR_INVALID, "conv1d_bwd: dw and its partial sums go together");
   if ((x_next == nullptr) != (dy_next == nullptr))
     return fail(MEK_ERR_INVALID, "conv1d_bwd: the continuation rows of x and of dy go together");
-  if (int rc = check_conv("conv1d_bwd", tokens, channels, 1)) return rc;
+  if (int rc = check_conv("conv1d_bwd", tokens, channels, 1, {x, x_prev, x_next, dy, dy_next, dx})) return rc;
   const ConvPlan plan = conv_plan(tokens);
   constexpr int kBwdCh = 4;  // channels per thread of the backward kernel
   const dim3 grid(plan.runs, (channels + 256 * kBwdCh - 1) / (256 * kBwdCh));
