@@ -12,8 +12,8 @@
 //
 // Arithmetic on packed pairs of FP32 (half the instructions; a row of 16 elements a thread took 427 of them scalar, which
 // bounded it), rows of a whole block streamed by bulk copies, narrow rows side by side in a warp.  Measured, bf16:
-// 32,768 x 4,096 forward 107 us = 5.0 TB/s, backward 154 us = 5.2 TB/s with the last sums (copy: 6.5); 16,384 x 8,192
-// with the checkpoint 135 + 140 us; 65,536 x 2,048 96 + 150.  What bounds it: the chain of a row's phases (wait, sums,
+// 32,768 x 4,096 forward 110 us = 4.9 TB/s, backward 155 us = 5.2 TB/s with the last sums (copy: 6.5); 16,384 x 8,192
+// with the checkpoint 139 + 149 us; 65,536 x 2,048 98 + 150.  What bounds it: the chain of a row's phases (wait, sums,
 // shuffles, barrier, output) with three blocks an SM (backward: two), at 60 % of the issue slots; below 512 columns the
 // instructions of a row.
 //
@@ -186,8 +186,11 @@ constexpr int kLnFwdBlocks = G <= 32 ? 5 : G == 128 ? 6 : G == 256 ? 3 : 1;
 template <int G>
 constexpr int kLnBwdBlocks = G <= 128 ? 4 : G == 256 ? 2 : 1;
 // The widest rows leave no registers for the parameters, which stay in shared memory: 32 elements a thread of 128 registers
-// (16-bit rows; with 1,024 threads of 64 registers the backward spilled and took 343 us for 8,192 x 16,384 instead of
-// 316), or 1,024 threads.
+// (16-bit rows; with 1,024 threads of 64 registers the backward took 343 us for 8,192 x 16,384, so it takes 332), or 1,024
+// threads.  Both spill in the backward all the same (bytes stored a thread): 278 - 348 with 512 threads, 576 - 596 where the
+// codes cannot be streamed; 222 - 516 with 1,024 threads of FP32; 60 - 686 with 1,024 threads and one element an access.
+// So do, of the narrower forms, FP32 rows of one warp x 16 elements (backward 280, forward 140) and, in the forward, odd
+// 16-bit rows side by side in a warp (122 - 134).
 template <int VEC, int G, int NV>
 constexpr bool kLnParamsShared = G == 1024 || NV * VEC == 32;
 

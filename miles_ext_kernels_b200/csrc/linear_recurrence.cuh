@@ -8,7 +8,8 @@
 // neighbouring channels), folds them to (A, B), and the warps' pairs chain through shared memory.  Between tiles the
 // state travels through a word (A, B) per tile and channel in global memory: a block publishes its tile's pair, looks
 // back over its predecessors' words for the nearest one that already stands for a state, folds forward from it,
-// publishes its own state and only then goes over its tokens (still on chip) a second time.
+// publishes its own state and only then goes over its tokens (still on chip) a second time: a single-pass scan with
+// decoupled look-back (D. Merrill, M. Garland, 2016).
 //
 // The tokens come by TMA, a box of 16 tokens x 64 channels per warp and tensor, and the outputs leave the same way from
 // the place of the inputs: no thread computes an address per token (which took more instructions than the recurrence
@@ -23,13 +24,14 @@
 //
 // Tiles are taken from a counter in the order of time (all channels' first tiles, then all second ones, ...), so a
 // tile's predecessors have always been taken before it by a block that is running or done: no wait can be for good.
-// Every wait is bounded all the same (one second); the carried state is then NaN.
+// Every wait is bounded all the same (one second); what it leaves unknown -- the warp's tokens, the carried state, all that
+// follows from them inside their sequence -- is then NaN.
 //
-// Measured at 4 x 4,096 tokens x 4,096 channels, bf16 with FP32 gates: forward 99 us = 5.4 TB/s, backward 184 us = 5.1
-// TB/s (copy: 6.5).  What bounds it: an SM holds four tiles (three in the backward), with its shared memory and its
-// registers both full, for 12,400 cycles each -- the number from the counter 1,750, the boxes from L2 1,700, the walk
-// 2,400, the warps' pairs 1,100, the look-back 2,600, prefixes 600, the second pass 1,400, the store 850 -- at 56 % of the
-// issue slots.  Tried and slower: blocks that stay and draw their next number early (235 -> 277 us at twice the
+// Measured at 4 x 4,096 tokens x 4,096 channels, bf16 with FP32 gates: forward 97 us = 5.5 TB/s, backward 184 - 194 us =
+// 4.8 - 5.1 TB/s (copy: 6.5).  What bounds it: an SM holds four tiles (three in the backward), with its shared memory and
+// its registers both full, for about 12,400 cycles each -- the number from the counter 1,750, the boxes from L2 1,700, the
+// walk 2,400, the warps' pairs 1,100, the look-back 2,600, prefixes 600, the second pass 1,400, the store 850 (stamps of
+// the forward before the votes on growth) -- at 61 % of the issue slots.  Tried and slower: blocks that stay and draw their next number early (235 -> 277 us at twice the
 // tokens: a tile waits behind its block's present one, and its chain behind it); four or sixteen warps a block (forward
 // 250 / 278, and 492 / 328 for one long chain on 512 channels instead of 334); decays in registers (267, spills);
 // scalar arithmetic (276).
